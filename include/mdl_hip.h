@@ -656,6 +656,72 @@ uint32_t mdl_update_classes(const mdl_update* updates_host, int32_t num_updates)
 int mdl_grouped_rowwise_adagrad(const mdl_update* updates, const mdl_update* updates_host,
                                 int32_t num_updates, float eps, int32_t* error_count, void* stream);
 
+/* ----------------------------------------------------------- attention --- */
+
+/*
+ * Attention over histories: a sliding window, first tokens that stay visible,
+ * a learned relative position bias by buckets, heads that share keys.
+ *
+ * q [batch, q_len, q_heads, head_dim], k and v [batch, k_len, kv_heads,
+ * head_dim] with any element strides over batch, row and head (head_dim
+ * contiguous); query head h reads key head h / (q_heads / kv_heads).  Query
+ * row r stands at column c = r + k_len - q_len.  first = the row's first
+ * unmasked column.  Column j is visible to c when mask[j] and mask[c], j <= c,
+ * and c - j < window or j < first + sinks.
+ *   x = scale * q.k + bias_table[bucket(c - j), h]
+ *   out = sum over visible j of softmax(x) v; zeros when none is visible.
+ * Masked rows of q, k and v are not read (any value may lie there).  The bias
+ * of a visible key may be -infinity (hides the key) or any finite value.
+ * bucket(d) = number of bucket_starts (ascending) at or below d.
+ */
+typedef struct mdl_attention {
+  const void* q;
+  const void* k;
+  const void* v;
+  const uint8_t* mask;           /* [batch, k_len] bytes, rows mask_row apart; NULL: all unmasked */
+  const void* bias_table;        /* [num_buckets, q_heads], contiguous; NULL: no bias */
+  const int32_t* bucket_starts;  /* device, num_buckets - 1 distances at which buckets 1, 2, ... begin */
+  int64_t batch, q_len, k_len;   /* q_len <= k_len */
+  int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head, mask_row;  /* element strides */
+  int64_t window;                /* <= 0: every earlier column */
+  int64_t sinks;
+  int32_t q_heads, kv_heads, head_dim, dtype;  /* head_dim 1..128 */
+  int32_t table_dtype, num_buckets;
+  int32_t distances;             /* last bucket's start + 1, at most 2049 */
+  float scale;                   /* > 0 */
+} mdl_attention;
+
+/* The mask as bits, each row's first unmasked column and the bias by
+ * distance, made once for the forward and backward of one call. */
+size_t mdl_attention_prepared_bytes(const mdl_attention* call);
+int mdl_attention_prepare(const mdl_attention* call, void* prepared, size_t prepared_bytes, void* stream);
+
+/* out: [batch, q_len, q_heads, head_dim] contiguous (dtype).  stats (NULL
+ * without a backward): float [batch, q_heads, q_len, 2], each row's largest
+ * score divided by scale and log2 of its softmax sum. */
+int mdl_attention_forward(const mdl_attention* call, const void* prepared, void* out, float* stats, void* stream);
+
+/*
+ * Gradients of q, k, v (contiguous, laid out as q, k and v; dtype) and, when
+ * grad_table is not NULL, of the bias table (table_dtype, contiguous), from
+ * the gradient of out (element strides; head_dim contiguous), the forward's
+ * out and stats.  Sums run in a fixed order: equal inputs give equal bits.
+ */
+typedef struct mdl_attention_grads {
+  const void* out;
+  const float* stats;
+  const void* grad_out;
+  int64_t grad_batch, grad_row, grad_head;
+  void* grad_q;
+  void* grad_k;
+  void* grad_v;
+  void* grad_table;
+} mdl_attention_grads;
+
+size_t mdl_attention_backward_workspace_bytes(const mdl_attention* call);
+int mdl_attention_backward(const mdl_attention* call, const void* prepared, const mdl_attention_grads* grads,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -100,6 +100,23 @@ assert CHUNK_DTYPE.itemsize == 16
 assert SPAN_DTYPE.itemsize == 32
 assert TABLE_DTYPE.itemsize == 48
 
+ATTENTION_DTYPE = np.dtype(
+    [(name, "<u8") for name in ("q", "k", "v", "mask", "bias_table", "bucket_starts")]
+    + [(name, "<i8") for name in (
+        "batch", "q_len", "k_len", "q_batch", "q_row", "q_head", "k_batch", "k_row", "k_head", "v_batch", "v_row",
+        "v_head", "mask_row", "window", "sinks")]
+    + [(name, "<i4") for name in (
+        "q_heads", "kv_heads", "head_dim", "dtype", "table_dtype", "num_buckets", "distances")]
+    + [("scale", "<f4")]
+)
+ATTENTION_GRADS_DTYPE = np.dtype(
+    [(name, "<u8") for name in ("out", "stats", "grad_out")]
+    + [(name, "<i8") for name in ("grad_batch", "grad_row", "grad_head")]
+    + [(name, "<u8") for name in ("grad_q", "grad_k", "grad_v", "grad_table")]
+)
+assert ATTENTION_DTYPE.itemsize == 200
+assert ATTENTION_GRADS_DTYPE.itemsize == 80
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -174,6 +191,11 @@ SIGNATURES: dict[str, tuple] = {
     "mdl_backward_pad": (_I32, [_P, _I32, _P, _P, _P, _P, _P, _I64, _P]),
     "mdl_update_classes": (_U32, [_P, _I32]),
     "mdl_grouped_rowwise_adagrad": (_I32, [_P, _P, _I32, _F, _P, _P]),
+    "mdl_attention_prepared_bytes": (_SZ, [_P]),
+    "mdl_attention_prepare": (_I32, [_P, _P, _SZ, _P]),
+    "mdl_attention_forward": (_I32, [_P, _P, _P, _P, _P]),
+    "mdl_attention_backward_workspace_bytes": (_SZ, [_P]),
+    "mdl_attention_backward": (_I32, [_P, _P, _P, _P, _SZ, _P]),
     "mdl_rowwise_adagrad": (
         _I32,
         [_P, _I32, _I64, _I32, _I64, _P, _P, _I64, _P, _I32, _I64, _F, _F, _P, _P],

@@ -6,7 +6,8 @@ is not needed to build them):
   ``mdl_amd/csrc/Makefile``);
 * ``libmdl_torch.so``: the PyTorch-ROCm extension that defines the
   ``mdl_hip`` torch.library operators over that C ABI (g++ against the
-  installed torch's headers and libraries, ``mdl_amd/csrc/torch_ops.cpp``).
+  installed torch's headers and libraries, ``mdl_amd/csrc/torch_ops.cpp`` and
+  ``history_ops.cpp``).
 """
 
 from __future__ import annotations
@@ -34,29 +35,41 @@ def build_hip(jobs: int | None = None, force: bool = True) -> Path:
     return out
 
 
-def torch_extension_command(out: Path) -> list[str]:
-    """The g++ line of libmdl_torch.so: torch's headers and ABI, HIP's
-    headers (for the current-stream API), linked against torch, c10_hip and
-    libmdl_hip.so (found next to it at run time)."""
+TORCH_SOURCES = ("torch_ops.cpp", "history_ops.cpp")
+
+
+def torch_extension_commands(out: Path) -> tuple[list[list[str]], list[str]]:
+    """The g++ lines of libmdl_torch.so, one per source and the link: torch's
+    headers and ABI, HIP's headers (for the current-stream API), linked
+    against torch, c10_hip and libmdl_hip.so (found next to it at run time)."""
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
-    cmd += [f"-I{p}" for p in include_paths()] + [f"-I{ROCM / 'include'}"]
-    cmd += [str(CSRC / "torch_ops.cpp"), "-o", str(out)]
-    cmd += [f"-L{p}" for p in library_paths()] + [f"-L{PKG}"]
-    cmd += ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-lmdl_hip", "-Wl,-rpath,$ORIGIN"]
-    cmd += [f"-Wl,-rpath,{p}" for p in library_paths()]
-    return cmd
+    objects = CSRC.parents[1] / "_build" / "torch"
+    objects.mkdir(parents=True, exist_ok=True)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1",
+             "-DUSE_ROCM=1"]
+    flags += [f"-I{p}" for p in include_paths()] + [f"-I{ROCM / 'include'}"]
+    built = [(CSRC / name, objects / name.replace(".cpp", ".o")) for name in TORCH_SOURCES]
+    compiles = [["g++", *flags, "-c", str(source), "-o", str(obj)] for source, obj in built]
+    link = ["g++", "-shared", *(str(obj) for _, obj in built), "-o", str(out)]
+    link += [f"-L{p}" for p in library_paths()] + [f"-L{PKG}"]
+    link += ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-lmdl_hip", "-Wl,-rpath,$ORIGIN"]
+    link += [f"-Wl,-rpath,{p}" for p in library_paths()]
+    return compiles, link
 
 
 def build_torch_extension() -> Path:
     out = PKG / "libmdl_torch.so"
     tmp = out.with_suffix(".so.tmp")
-    subprocess.run(torch_extension_command(tmp), check=True)
+    compiles, link = torch_extension_commands(tmp)
+    running = [subprocess.Popen(cmd) for cmd in compiles]
+    for cmd, code in [(cmd, p.wait()) for cmd, p in zip(compiles, running)]:
+        if code:
+            raise subprocess.CalledProcessError(code, cmd)
+    subprocess.run(link, check=True)
     tmp.replace(out)
     return out
 

@@ -1,0 +1,396 @@
+// Attention over histories, forward: a sliding window, first tokens that stay
+// visible, and a learned relative position bias.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax:
+// a block owns 128 query rows of one head (32 per wave) and walks key tiles
+// that hold a visible column.  Per tile a wave makes x^T = K q^T (its queries
+// are the result's columns, so a query's statistics are one value per lane),
+// p = exp2(c2 x - c2 m), and out^T += V^T p^T.  Out is divided by l at the
+// end; a query without a visible key gets zeros.
+#include "attention.cuh"
+
+namespace mdl {
+
+// ------------------------------------------------------------------- prepare --
+//
+// What a call's kernels read instead of the mask and the bias table: the
+// mask's columns as bits, the first unmasked column of a row, and every
+// head's bias by distance, divided by the scale.
+
+template <typename TB>
+__device__ __forceinline__ float table_value(const TB* p) {
+  if constexpr (sizeof(TB) == 2) return bf16_to_f32(*p);
+  else return *p;
+}
+
+// Bucket of a distance: the number of starts at or below it.
+__device__ __forceinline__ int bucket_of_distance(const int32_t* starts, int buckets, int d) {
+  int lo = 0, hi = buckets - 1;  // starts[0 .. hi) of bucket 1 ..
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= d) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct PrepareCall {
+  const uint8_t* mask;
+  int64_t mask_row;
+  const void* table;
+  const int32_t* starts;
+  uint64_t* words;
+  int32_t* first;
+  float* bias;
+  int64_t words_row;
+  int32_t batch, k_len, heads, buckets, distances;
+  int32_t table_f32;
+  float inv_scale;
+};
+
+__global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
+  const int wave = threadIdx.x / kWave;
+  int64_t block = blockIdx.x;
+  if (a.mask) {
+    if (block < a.batch) {
+      __shared__ int firsts[4];
+      const uint8_t* row = a.mask + block * a.mask_row;
+      uint64_t* words = a.words + block * a.words_row;
+      int first = a.k_len;
+      for (int w = wave; w < a.words_row; w += 4) {
+        const int col = 64 * w + lane_id();
+        const uint64_t word = __ballot(col < a.k_len && row[col] != 0);
+        if (word && first == a.k_len) first = 64 * w + __builtin_ctzll(word);
+        if (lane_id() == 0) words[w] = word;
+      }
+      if (lane_id() == 0) firsts[wave] = first;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int i = 1; i < 4; ++i) first = firsts[i] < first ? firsts[i] : first;
+        a.first[block] = first;
+      }
+      return;
+    }
+    block -= a.batch;
+  }
+  const int64_t i = block * 256 + threadIdx.x;
+  if (i >= (int64_t)a.heads * a.distances) return;
+  const int h = (int)(i / a.distances), d = (int)(i % a.distances);
+  const int64_t at = (int64_t)bucket_of_distance(a.starts, a.buckets, d) * a.heads + h;
+  const float v = a.table_f32 ? table_value(static_cast<const float*>(a.table) + at)
+                              : table_value(static_cast<const bf16_t*>(a.table) + at);
+  float x = v * a.inv_scale;
+  // an infinite bias hides a key; a finite one never does, however low
+  if (__builtin_isfinite(v)) x = fminf(fmaxf(x, kLowScore), -kLowScore);
+  a.bias[i] = x;
+}
+
+// ------------------------------------------------------------------- forward --
+
+// Raises of a row's maximum below this many powers of two are not applied
+// (p stays below 2^8): most tiles then skip the rescaling of out.
+constexpr float kLazyRaise = 8.f;
+
+template <typename T, int DP, bool kVec>
+__global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCall a, T* out, float2* stats) {
+  using F = Frags<T>;
+  using Stage = TileStage<T, DP, kVec>;
+  constexpr int TK = F::kTile, LD = Stage::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;
+  constexpr int kBias = kAttnRows + TK;  // distances of a block and a tile
+  extern __shared__ __align__(16) char smem[];
+  T* lds = reinterpret_cast<T*>(smem);                     // [2][K, V][TK][LD]
+  float* lds_bias = reinterpret_cast<float*>(lds + 4 * TK * LD);  // [2][kBias]
+
+  const int blocks_q = (a.q_len + kAttnRows - 1) / kAttnRows;
+  int64_t id = xcd_block(blockIdx.x, gridDim.x);
+  // last rows first: without a window they walk the most tiles
+  const int qb = blocks_q - 1 - (int)(id % blocks_q);
+  id /= blocks_q;
+  const int head = (int)(id % a.q_heads), b = (int)(id / a.q_heads);
+  const int kv = head / (a.q_heads / a.kv_heads);
+  const T* kp = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
+  const float* bias = a.bias ? a.bias + (int64_t)head * a.distances : nullptr;
+
+  const int off = a.k_len - a.q_len;
+  const int wave = threadIdx.x / kWave, l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int r0 = qb * kAttnRows;
+  const int r_end = r0 + kAttnRows < a.q_len ? r0 + kAttnRows : a.q_len;
+  const int row = r0 + 32 * wave + l32, c = row + off;
+  KeyWalk walk(a, b, TK, r0 + off, r_end - 1 + off);
+  const int wc_lo = r0 + 32 * wave + off;  // the wave's columns
+  const uint32_t q_bits = wc_lo - off < a.q_len ? columns32(a, walk.words, wc_lo) : 0;
+  const bool live = (q_bits >> l32) & 1;
+
+  typename F::Frag q[kSteps];
+  load_own_row<T, DP, kVec>(static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head + (int64_t)row * a.q_row,
+                            live, a.dim, q);
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = (f32x16)(0.f);
+  float m = kNoScore, mneg = -(kNoScore * a.c2), l = 0.f;
+  const float lazy = kLazyRaise / a.c2;
+
+  const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
+  Stage ks, vs;
+  float bias_next = 0.f;
+  auto fetch = [&](int t, uint64_t bits) {
+    ks.load(kp, a.k_row, t * TK, bits, a.dim);
+    vs.load(vp, a.v_row, t * TK, bits, a.dim);
+    if (bias && threadIdx.x < kBias) {
+      // lds_bias[i]: the distance of query i' and key k' with k' - i' = i - (rows - 1)
+      int d = r0 + off - t * TK + kAttnRows - 1 - (int)threadIdx.x;
+      d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
+      bias_next = bias[d];
+    }
+  };
+  uint64_t bits = 0, bits_next = 0;
+  int t = walk.begin(a, &bits);
+  if (t <= walk.last_tile) fetch(t, bits);
+  int buf = 0;
+  while (t <= walk.last_tile) {
+    T* lk = lds + buf * 2 * TK * LD;
+    T* lv = lk + TK * LD;
+    float* lb = lds_bias + buf * kBias;
+    ks.store(lk);
+    vs.store(lv);
+    if (bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
+    const int t_next = walk.seek(a, t + 1, &bits_next);
+    if (t_next <= walk.last_tile) fetch(t_next, bits_next);
+    __syncthreads();
+
+    const int j0 = t * TK, j1 = j0 + TK - 1;
+    const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
+    if (seen) {
+      f32x16 x[kSubs];
+      // distances of the wave and the tile all in the last bucket, or none told apart
+      const bool flat = !bias || wc_lo - j1 >= a.distances - 1;
+      const float flat_bias = bias ? lb[kAttnRows - 32 - 32 * wave] : 0.f;
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) {
+        if (flat) {
+          x[s] = (f32x16)(flat_bias);
+        } else {
+          const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[s][i] = from[8 * (i >> 2) + (i & 3)];
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d)
+          x[s] = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x[s]);
+      }
+      const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
+                         wc_lo + 31 - j0 < a.window;
+      if (!whole) {
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s) {
+          uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
+          vis >>= 4 * half;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[s][i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[s][i], -INFINITY);
+        }
+      }
+      float top = x[0][0];
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, x[s][i]);
+      top = max_halves(top);
+      if (__any(top > m + lazy)) {
+        const float up = fmaxf(m, top);
+        const float shrink = exp2_fast((m - up) * a.c2);
+        m = up;
+        mneg = -(m * a.c2);
+        l *= shrink;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) acc[i] *= shrink;
+      }
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[s][i] = exp2_fast(__builtin_fmaf(x[s][i], a.c2, mneg));
+          l += x[s][i];
+        }
+        // the weights take the element type for the second product; their sum does not
+#pragma unroll
+        for (int p = 0; p < 32 / F::kStep; ++p) {
+          const typename F::Frag pf = F::from_result(x[s], p);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt)
+            acc[dt] = F::mma(F::load_t(lv + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), pf, acc[dt]);
+        }
+      }
+    }
+    t = t_next;
+    bits = bits_next;
+    buf ^= 1;
+  }
+
+  l = sum_halves(l);
+  if (row < a.q_len) {
+    store_result_row<T, DP>(out + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim, acc,
+                            l > 0.f ? 1.f / l : 0.f, a.dim);
+    if (stats && half == 0) {
+      // log2 of the sum at the unrounded c2 m; +inf makes every weight of an empty row 0
+      const float ll = l > 0.f ? log2f(l) - __builtin_fmaf(m, a.c2, mneg) : INFINITY;
+      stats[((int64_t)b * a.q_heads + head) * a.q_len + row] = make_float2(l > 0.f ? m : 0.f, ll);
+    }
+  }
+}
+
+template <typename T, int DP>
+size_t forward_lds() {
+  using F = Frags<T>;
+  return (size_t)4 * F::kTile * (DP + F::kPad) * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
+}
+
+template <typename T, int DP, bool kVec>
+int launch_forward(const AttnCall& a, void* out, float2* stats, hipStream_t s) {
+  const int64_t blocks = (int64_t)((a.q_len + kAttnRows - 1) / kAttnRows) * a.q_heads * a.batch;
+  if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_forward: too many rows");
+  const size_t lds = forward_lds<T, DP>();
+  const auto kernel = attention_forward_kernel<T, DP, kVec>;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, static_cast<T*>(out), stats);
+  MDL_CHECK_LAUNCH("attention_forward_kernel");
+  return MDL_OK;
+}
+
+// ---------------------------------------------------------------- host side --
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+int64_t mask_words_row(const mdl_attention& a) { return (a.k_len + 63) / 64 + 1; }
+
+// Where a prepared call's parts lie.
+struct PrepareLayout {
+  size_t words = 0, first = 0, bias = 0, bytes = 0;
+  explicit PrepareLayout(const mdl_attention& a) {
+    size_t at = 0;
+    if (a.mask) {
+      words = at;
+      at = align256(at + (size_t)a.batch * mask_words_row(a) * 8);
+      first = at;
+      at = align256(at + (size_t)a.batch * 4);
+    }
+    if (a.bias_table) {
+      bias = at;
+      at = align256(at + (size_t)a.q_heads * a.distances * 4);
+    }
+    bytes = at;
+  }
+};
+
+int attention_check(const mdl_attention* a, const char* what) {
+  const std::string w(what);
+  if (!a) return fail(MDL_ERR_INVALID, w + ": null descriptor");
+  if (a->batch < 0 || a->q_len < 0 || a->k_len < a->q_len)
+    return fail(MDL_ERR_INVALID, w + ": needs batch >= 0 and 0 <= q_len <= k_len");
+  if (a->batch > 0x7fffffff || a->k_len > 0x3fffffff) return fail(MDL_ERR_UNSUPPORTED, w + ": too many rows");
+  if (a->q_heads <= 0 || a->kv_heads <= 0 || a->q_heads % a->kv_heads)
+    return fail(MDL_ERR_INVALID, w + ": q_heads must be a positive multiple of kv_heads");
+  if (a->head_dim <= 0 || a->head_dim > 128) return fail(MDL_ERR_UNSUPPORTED, w + ": head_dim must be 1..128");
+  if (a->dtype != MDL_F32 && a->dtype != MDL_BF16) return fail(MDL_ERR_INVALID, w + ": dtype");
+  if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(MDL_ERR_INVALID, w + ": scale must be positive");
+  if (a->sinks < 0) return fail(MDL_ERR_INVALID, w + ": sinks must not be negative");
+  if (a->bias_table) {
+    if (a->table_dtype != MDL_F32 && a->table_dtype != MDL_BF16) return fail(MDL_ERR_INVALID, w + ": table_dtype");
+    if (a->num_buckets < 1 || (a->num_buckets > 1 && !a->bucket_starts) || a->distances < 1)
+      return fail(MDL_ERR_INVALID, w + ": bias buckets");
+    if (a->distances > kMaxDistances || a->num_buckets > 1024)
+      return fail(MDL_ERR_UNSUPPORTED, w + ": bias buckets must begin at distances up to 2048, at most 1024 of them");
+  }
+  if (a->batch * a->q_len > 0 && (!a->q || !a->k || !a->v)) return fail(MDL_ERR_INVALID, w + ": null pointer");
+  return MDL_OK;
+}
+
+AttnCall attention_call(const mdl_attention& a, const void* prepared) {
+  const char* p = static_cast<const char*>(prepared);
+  const PrepareLayout lay(a);
+  AttnCall c{};
+  c.q = a.q; c.k = a.k; c.v = a.v;
+  c.q_batch = a.q_batch; c.q_row = a.q_row; c.q_head = a.q_head;
+  c.k_batch = a.k_batch; c.k_row = a.k_row; c.k_head = a.k_head;
+  c.v_batch = a.v_batch; c.v_row = a.v_row; c.v_head = a.v_head;
+  if (a.mask) {
+    c.words = reinterpret_cast<const uint64_t*>(p + lay.words);
+    c.first = reinterpret_cast<const int32_t*>(p + lay.first);
+    c.words_row = mask_words_row(a);
+  }
+  if (a.bias_table) c.bias = reinterpret_cast<const float*>(p + lay.bias);
+  c.batch = (int32_t)a.batch; c.q_len = (int32_t)a.q_len; c.k_len = (int32_t)a.k_len;
+  c.q_heads = a.q_heads; c.kv_heads = a.kv_heads; c.dim = a.head_dim;
+  c.distances = a.bias_table ? a.distances : 0;
+  c.window = (int32_t)(a.window > 0 && a.window < a.k_len ? a.window : a.k_len);
+  // without a window every earlier column is visible as it is
+  c.sinks = (int32_t)(c.window >= c.k_len ? 0 : (a.sinks < a.k_len ? a.sinks : a.k_len));
+  c.scale = a.scale;
+  c.c2 = (float)((double)a.scale * 1.4426950408889634);
+  return c;
+}
+
+bool attention_vectors(const mdl_attention& a) {
+  const int64_t e = a.dtype == MDL_BF16 ? 8 : 4;
+  auto whole = [&](const void* p, int64_t b, int64_t r, int64_t h) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && b % e == 0 && r % e == 0 && h % e == 0;
+  };
+  return a.head_dim % e == 0 && whole(a.q, a.q_batch, a.q_row, a.q_head) && whole(a.k, a.k_batch, a.k_row, a.k_head) &&
+         whole(a.v, a.v_batch, a.v_row, a.v_head);
+}
+
+int allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return MDL_OK;
+  return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                   "hipFuncSetAttribute");
+}
+
+}  // namespace mdl
+
+using namespace mdl;
+
+extern "C" {
+
+size_t mdl_attention_prepared_bytes(const mdl_attention* a) { return a ? PrepareLayout(*a).bytes : 0; }
+
+int mdl_attention_prepare(const mdl_attention* a, void* prepared, size_t prepared_bytes, void* stream) {
+  if (int rc = attention_check(a, "mdl_attention_prepare")) return rc;
+  const PrepareLayout lay(*a);
+  if (lay.bytes == 0 || a->batch == 0 || a->q_len == 0) return MDL_OK;
+  if (!prepared || prepared_bytes < lay.bytes)
+    return fail(MDL_ERR_WORKSPACE, "mdl_attention_prepare: prepared buffer too small");
+  char* p = static_cast<char*>(prepared);
+  PrepareCall c{};
+  c.mask = a->mask;
+  c.mask_row = a->mask_row;
+  c.table = a->bias_table;
+  c.starts = a->bucket_starts;
+  c.words = reinterpret_cast<uint64_t*>(p + lay.words);
+  c.first = reinterpret_cast<int32_t*>(p + lay.first);
+  c.bias = reinterpret_cast<float*>(p + lay.bias);
+  c.words_row = mask_words_row(*a);
+  c.batch = (int32_t)a->batch;
+  c.k_len = (int32_t)a->k_len;
+  c.heads = a->q_heads;
+  c.buckets = a->num_buckets;
+  c.distances = a->bias_table ? a->distances : 0;
+  c.table_f32 = a->table_dtype == MDL_F32;
+  c.inv_scale = 1.f / a->scale;
+  const int64_t blocks = (a->mask ? a->batch : 0) + ((int64_t)c.heads * c.distances + 255) / 256;
+  hipLaunchKernelGGL(attention_prepare_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), c);
+  MDL_CHECK_LAUNCH("attention_prepare_kernel");
+  return MDL_OK;
+}
+
+int mdl_attention_forward(const mdl_attention* a, const void* prepared, void* out, float* stats, void* stream) {
+  if (int rc = attention_check(a, "mdl_attention_forward")) return rc;
+  if (a->batch == 0 || a->q_len == 0) return MDL_OK;
+  if (!out || (PrepareLayout(*a).bytes && !prepared))
+    return fail(MDL_ERR_INVALID, "mdl_attention_forward: null pointer");
+  const AttnCall c = attention_call(*a, prepared);
+  return for_attention(*a, attention_vectors(*a), [&]<typename T, int DP, bool kVec>() {
+    return launch_forward<T, DP, kVec>(c, out, reinterpret_cast<float2*>(stats), as_stream(stream));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,565 @@
+// Gradients of the history attention.
+//
+// With p the forward's weights (made again from q, k and the saved row
+// statistics), dP = dO . v and delta = sum p dP = dO . out of a row:
+//   dS = p (dP - delta),  dq = scale sum_k dS k,  dk = scale sum_q dS q,
+//   dv = sum_q p dO,      dbias[bucket] = sum of dS over the bucket's places.
+// Two kernels, so that every sum has one owner and a fixed order: one walks
+// the keys of 128 queries (dq, delta and the bias), one the queries of 128
+// keys (dk and dv, over all heads that share the keys).  Making the weights
+// twice costs seven products instead of five; adding dq across blocks
+// instead would need atomics, whose order changes results.
+#include "attention.cuh"
+
+namespace mdl {
+
+struct GradCall {
+  const void* out;
+  const float2* stats;
+  const void* grad_out;
+  int64_t g_batch, g_row, g_head;
+  void *dq, *dk, *dv;
+  float* delta;         // [B, Hq, Lq]
+  const int32_t* starts;
+  int32_t buckets;
+  float* bias_partial;  // [Hq, B * blocks_q, buckets]; NULL: no bias gradient
+  float* far_partial;   // [B, Hkv, far_chunks, sinks, 2, dim]; NULL: no far part
+  int32_t far_chunks;
+};
+
+constexpr int kSpare = 96;      // distances of one tile and wave past either end of the bias
+constexpr int kFarRows = 512;   // query rows of a block of the first tokens' far part
+
+// ------------------------------------------------- queries: dq, delta, bias --
+
+template <typename T, int DP, bool kVec>
+__global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall a, GradCall g) {
+  using F = Frags<T>;
+  using Stage = TileStage<T, DP, kVec>;
+  constexpr int TK = F::kTile, LD = Stage::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;
+  constexpr int kBias = kAttnRows + TK;
+  extern __shared__ __align__(16) char smem[];
+  T* lds = reinterpret_cast<T*>(smem);
+  float* lds_bias = reinterpret_cast<float*>(lds + 4 * TK * LD);
+  // bias gradient by distance: one array per wave and half wave, so that the
+  // lanes of one addition never meet and every array is added to in order
+  float* lds_sum = lds_bias + 2 * kBias;
+  const int n_sum = g.bias_partial ? a.distances + 2 * kSpare : 0;
+
+  const int blocks_q = (a.q_len + kAttnRows - 1) / kAttnRows;
+  int64_t id = xcd_block(blockIdx.x, gridDim.x);
+  const int qb = blocks_q - 1 - (int)(id % blocks_q);
+  id /= blocks_q;
+  const int head = (int)(id % a.q_heads), b = (int)(id / a.q_heads);
+  const int kv = head / (a.q_heads / a.kv_heads);
+  const T* kp = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
+  const float* bias = a.bias ? a.bias + (int64_t)head * a.distances : nullptr;
+
+  const int off = a.k_len - a.q_len;
+  const int wave = threadIdx.x / kWave, l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int r0 = qb * kAttnRows;
+  const int r_end = r0 + kAttnRows < a.q_len ? r0 + kAttnRows : a.q_len;
+  const int row = r0 + 32 * wave + l32, c = row + off;
+  KeyWalk walk(a, b, TK, r0 + off, r_end - 1 + off);
+  const int wc_lo = r0 + 32 * wave + off;
+  const uint32_t q_bits = wc_lo - off < a.q_len ? columns32(a, walk.words, wc_lo) : 0;
+  const bool live = (q_bits >> l32) & 1;
+
+  typename F::Frag q[kSteps], go[kSteps];
+  load_own_row<T, DP, kVec>(static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head + (int64_t)row * a.q_row,
+                            live, a.dim, q);
+  load_own_row<T, DP, kVec>(
+      static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head + (int64_t)row * g.g_row, live, a.dim, go);
+  float m = 0.f, ll = INFINITY, delta = 0.f;
+  {
+    const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + row;
+    typename F::Frag o[kSteps];
+    load_own_row<T, DP, kVec>(static_cast<const T*>(g.out) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim,
+                              live, a.dim, o);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int i = 0; i < F::kElems; ++i) delta += (float)o[s][i] * (float)go[s][i];
+    delta = sum_halves(delta);
+    if (row < a.q_len) {
+      const float2 st = g.stats[at];
+      m = st.x;
+      ll = st.y;
+      if (half == 0) g.delta[at] = delta;
+    }
+  }
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = (f32x16)(0.f);
+  float flat_sum = 0.f;
+  float* my_sum = lds_sum + (2 * wave + half) * n_sum;
+  for (int i = threadIdx.x; i < 8 * n_sum; i += kAttnThreads) lds_sum[i] = 0.f;
+
+  const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
+  Stage ks, vs;
+  float bias_next = 0.f;
+  auto fetch = [&](int t, uint64_t bits) {
+    ks.load(kp, a.k_row, t * TK, bits, a.dim);
+    vs.load(vp, a.v_row, t * TK, bits, a.dim);
+    if (bias && threadIdx.x < kBias) {
+      int d = r0 + off - t * TK + kAttnRows - 1 - (int)threadIdx.x;
+      d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
+      bias_next = bias[d];
+    }
+  };
+  uint64_t bits = 0, bits_next = 0;
+  int t = walk.begin(a, &bits);
+  if (t <= walk.last_tile) fetch(t, bits);
+  int buf = 0;
+  while (t <= walk.last_tile) {
+    T* lk = lds + buf * 2 * TK * LD;
+    T* lv = lk + TK * LD;
+    float* lb = lds_bias + buf * kBias;
+    ks.store(lk);
+    vs.store(lv);
+    if (bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
+    const int t_next = walk.seek(a, t + 1, &bits_next);
+    if (t_next <= walk.last_tile) fetch(t_next, bits_next);
+    __syncthreads();
+
+    const int j0 = t * TK, j1 = j0 + TK - 1;
+    const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
+    if (seen) {
+      const bool flat = !bias || wc_lo - j1 >= a.distances - 1;
+      const float flat_bias = bias ? lb[kAttnRows - 32 - 32 * wave] : 0.f;
+      const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
+                         wc_lo + 31 - j0 < a.window;
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) {
+        f32x16 x, dp = (f32x16)(-delta);
+        if (flat) {
+          x = (f32x16)(flat_bias - m);
+        } else {
+          const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = from[8 * (i >> 2) + (i & 3)] - m;
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          x = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x);
+          dp = F::mma(load_frag(lv + nat + 32 * s * LD + d * F::kStep), go[d], dp);
+        }
+        if (!whole) {
+          uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
+          vis >>= 4 * half;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, -ll)) * dp[i];
+        if (n_sum) {
+          if (flat) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) flat_sum += x[i];
+          } else {
+            float* at = my_sum + (c - j0 - 32 * s - 4 * half + kSpare);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lds_add(at - (8 * (i >> 2) + (i & 3)), x[i]);
+          }
+        }
+        // dS takes the element type for the product with k
+#pragma unroll
+        for (int p = 0; p < 32 / F::kStep; ++p) {
+          const typename F::Frag pf = F::from_result(x, p);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt)
+            acc[dt] = F::mma(F::load_t(lk + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), pf, acc[dt]);
+        }
+      }
+    }
+    t = t_next;
+    bits = bits_next;
+    buf ^= 1;
+  }
+  if (row < a.q_len)
+    store_result_row<T, DP>(static_cast<T*>(g.dq) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim, acc,
+                            a.scale, a.dim);
+  if (!n_sum) return;
+
+  // the block's bias gradient by bucket
+  for (int s = 32; s >= 1; s >>= 1) flat_sum += __shfl_xor(flat_sum, s);
+  __syncthreads();
+  if (lane_id() == 0) lds_bias[wave] = flat_sum;
+  for (int i = threadIdx.x; i < n_sum; i += kAttnThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += lds_sum[w * n_sum + i];
+    lds_sum[i] = s;
+  }
+  __syncthreads();
+  float* partial = g.bias_partial + (((int64_t)head * a.batch + b) * blocks_q + qb) * g.buckets;
+  const int sub = threadIdx.x & 7;
+  for (int k = threadIdx.x >> 3; k < g.buckets; k += kAttnThreads / 8) {
+    const int lo = k == 0 ? 0 : g.starts[k - 1];
+    const int hi = k == g.buckets - 1 ? n_sum - kSpare : g.starts[k];
+    float s = 0.f;
+    for (int d = lo + sub; d < hi; d += 8) s += lds_sum[d + kSpare];
+    for (int x = 4; x >= 1; x >>= 1) s += __shfl_xor(s, x);
+    if (k == g.buckets - 1) s += (lds_bias[0] + lds_bias[1]) + (lds_bias[2] + lds_bias[3]);
+    if (sub == 0) partial[k] = s;
+  }
+}
+
+// grad_table[bucket, head]: the blocks' parts in order.  A block sums 8
+// buckets of one head, 32 threads each.
+template <typename TB>
+__global__ __launch_bounds__(256) void bias_partial_sum_kernel(const float* partial, int64_t parts, int buckets,
+                                                               int heads, TB* grad) {
+  __shared__ float smem[256];
+  const int head = blockIdx.y, k = blockIdx.x * 8 + (threadIdx.x & 7), part = threadIdx.x >> 3;
+  float s = 0.f;
+  if (k < buckets) {
+    const float* p = partial + (int64_t)head * parts * buckets + k;
+#pragma unroll 4
+    for (int64_t i = part; i < parts; i += 32) s += p[i * buckets];
+  }
+  smem[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x < 8 && k < buckets) {
+    double t = 0.;
+    for (int i = 0; i < 32; ++i) t += (double)smem[8 * i + threadIdx.x];
+    if constexpr (sizeof(TB) == 2) grad[(int64_t)k * heads + head] = f32_to_bf16((float)t);
+    else grad[(int64_t)k * heads + head] = (float)t;
+  }
+}
+
+// ---------------------------------------------------------- keys: dk and dv --
+
+// kFar: the pairs of the first tokens and the queries a window or more past
+// them.  Every query after a first token sees it, so a block of first tokens
+// alone would walk the whole row while the others walk one window; these
+// pairs are cut into kFarRows query rows a block instead, whose parts the
+// block that owns the keys adds in order.
+template <typename T, int DP, bool kVec, bool kFar>
+__global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCall a, GradCall g) {
+  using F = Frags<T>;
+  using Stage = TileStage<T, DP, kVec>;
+  constexpr int TQ = F::kTile, LD = Stage::kLd, kSteps = DP / F::kStep, kSubs = TQ / 32;
+  constexpr int kBias = kAttnRows + TQ;
+  extern __shared__ __align__(16) char smem[];
+  T* lds = reinterpret_cast<T*>(smem);                             // [2][Q, dO][TQ][LD]
+  float* lds_row = reinterpret_cast<float*>(lds + 4 * TQ * LD);    // [2][m, log2 sum, delta][TQ]
+  float* lds_bias = lds_row + 6 * TQ;                              // [2][kBias]
+
+  const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
+  const int key_blocks = ((kFar ? a.sinks : a.k_len) + kAttnRows - 1) / kAttnRows;
+  int64_t id = xcd_block(blockIdx.x, gridDim.x);
+  const int kb = (int)(id % key_blocks);  // first keys first: without a window they walk the most tiles
+  id /= key_blocks;
+  int chunk = 0;
+  if (kFar) {
+    chunk = (int)(id % g.far_chunks);
+    id /= g.far_chunks;
+  }
+  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
+  const uint64_t* words = a.words ? a.words + (int64_t)b * a.words_row : nullptr;
+  const int first = a.words ? a.first[b] : 0;
+  const int sink_end = first + a.sinks < a.k_len ? first + a.sinks : a.k_len;
+
+  const int wave = threadIdx.x / kWave, l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int k0 = (kFar ? first : 0) + kb * kAttnRows;
+  const int k_end = kFar ? sink_end : a.k_len;
+  const int jw = k0 + 32 * wave, j = jw + l32;
+  const uint32_t k_bits = columns32(a, words, jw) & low_bits(k_end - jw);
+  const bool live = (k_bits >> l32) & 1;
+
+  typename F::Frag kf[kSteps], vf[kSteps];
+  load_own_row<T, DP, kVec>(static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head + (int64_t)j * a.k_row, live,
+                            a.dim, kf);
+  load_own_row<T, DP, kVec>(static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head + (int64_t)j * a.v_row, live,
+                            a.dim, vf);
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = (f32x16)(0.f);
+
+  // query rows with a pair here
+  int r_lo, r_hi;
+  if (kFar) {
+    r_lo = chunk * kFarRows;
+    r_hi = r_lo + kFarRows - 1;
+    if (r_lo < k0 + a.window - off) r_lo = k0 + a.window - off;
+  } else {
+    r_lo = k0 - off;
+    r_hi = (k_end < k0 + kAttnRows ? k_end : k0 + kAttnRows) - 1 + a.window - 1 - off;
+  }
+  if (r_lo < 0) r_lo = 0;
+  if (r_hi > a.q_len - 1) r_hi = a.q_len - 1;
+  const int t_first = r_lo / TQ;
+  const int t_last = k0 < k_end && r_lo <= r_hi ? r_hi / TQ : -1;
+
+  const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
+  Stage qs, gs;
+  float2 stat_next = make_float2(0.f, INFINITY);
+  float delta_next = 0.f, bias_next = 0.f;
+  auto row_bits = [&](int t) {
+    const uint32_t lo = columns32(a, words, t * TQ + off);
+    if (TQ == 32) return (uint64_t)lo;
+    return lo | (uint64_t)columns32(a, words, t * TQ + off + 32) << 32;
+  };
+  // (head of the group, tile) from (share_, t) on with an unmasked query
+  auto seek = [&](int& hs, int& t, uint64_t& bits) {
+    for (; hs < share; ++hs, t = t_first)
+      for (; t <= t_last; ++t) {
+        bits = row_bits(t);
+        if (bits) return;
+      }
+  };
+  auto fetch = [&](int hs, int t, uint64_t bits) {
+    const int head = kv * share + hs;
+    qs.load(static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head, a.q_row, t * TQ, bits, a.dim);
+    gs.load(static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head, g.g_row, t * TQ, bits, a.dim);
+    if (threadIdx.x < TQ) {
+      const int r = t * TQ + (int)threadIdx.x;
+      const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + r;
+      stat_next = r < a.q_len ? g.stats[at] : make_float2(0.f, INFINITY);
+      delta_next = r < a.q_len ? g.delta[at] : 0.f;
+    }
+    if (a.bias && threadIdx.x < kBias) {
+      // lds_bias[i]: the distance of query q' and key k' with q' - k' = i - (rows - 1)
+      int d = t * TQ + off - k0 - (kAttnRows - 1) + (int)threadIdx.x;
+      d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
+      bias_next = a.bias[(int64_t)head * a.distances + d];
+    }
+  };
+
+  int hs = 0, t = t_first;
+  uint64_t bits = 0, bits_next = 0;
+  if (t_last < 0) hs = share;
+  seek(hs, t, bits);
+  if (hs < share) fetch(hs, t, bits);
+  int buf = 0;
+  while (hs < share) {
+    T* lq = lds + buf * 2 * TQ * LD;
+    T* lg = lq + TQ * LD;
+    float* lr = lds_row + buf * 3 * TQ;
+    float* lb = lds_bias + buf * kBias;
+    qs.store(lq);
+    gs.store(lg);
+    if (threadIdx.x < TQ) {
+      lr[threadIdx.x] = stat_next.x;
+      lr[TQ + threadIdx.x] = stat_next.y;
+      lr[2 * TQ + threadIdx.x] = delta_next;
+    }
+    if (a.bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
+    int hs_next = hs, t_next = t + 1;
+    seek(hs_next, t_next, bits_next);
+    if (hs_next < share) fetch(hs_next, t_next, bits_next);
+    __syncthreads();
+
+    const int c0 = t * TQ + off, c1 = c0 + TQ - 1;
+    const bool seen = k_bits && (kFar ? c1 >= jw + a.window : c1 >= jw && c0 - (jw + 31) < a.window);
+    if (seen) {
+      const bool flat = !a.bias || c0 - (jw + 31) >= a.distances - 1;
+      const float flat_bias = a.bias ? lb[kAttnRows - 32 - 32 * wave] : 0.f;
+      const bool whole = k_bits == ~0u && (TQ == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) &&
+                         (kFar ? c0 >= jw + 31 + a.window : c0 >= jw + 31 && c1 - jw < a.window);
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) {
+        f32x16 x, dp;
+        const float* rows = lr + 32 * s + 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[i] = -rows[8 * (i >> 2) + (i & 3)];
+          dp[i] = -rows[2 * TQ + 8 * (i >> 2) + (i & 3)];
+        }
+        if (flat) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] += flat_bias;
+        } else {
+          const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] += from[8 * (i >> 2) + (i & 3)];
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          x = F::mma(load_frag(lq + nat + 32 * s * LD + d * F::kStep), kf[d], x);
+          dp = F::mma(load_frag(lg + nat + 32 * s * LD + d * F::kStep), vf[d], dp);
+        }
+        if (!whole) {
+          const int col = c0 + 32 * s;
+          uint32_t vis = ~low_bits((kFar ? j + a.window : j) - col);
+          if (!kFar) vis &= low_bits(j + a.window - col);
+          vis = live ? vis & (uint32_t)(bits >> (32 * s)) : 0u;
+          vis >>= 4 * half;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, -rows[TQ + 8 * (i >> 2) + (i & 3)]));
+#pragma unroll
+        for (int p = 0; p < 32 / F::kStep; ++p) {
+          const typename F::Frag pf = F::from_result(x, p);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt)
+            dv[dt] = F::mma(F::load_t(lg + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), pf, dv[dt]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= dp[i];
+#pragma unroll
+        for (int p = 0; p < 32 / F::kStep; ++p) {
+          const typename F::Frag sf = F::from_result(x, p);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt)
+            dk[dt] = F::mma(F::load_t(lq + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), sf, dk[dt]);
+        }
+      }
+    }
+    hs = hs_next;
+    t = t_next;
+    bits = bits_next;
+    buf ^= 1;
+  }
+
+  if (kFar) {
+    if (j < k_end) {
+      float* part = g.far_partial +
+                    (((((int64_t)b * a.kv_heads + kv) * g.far_chunks + chunk) * a.sinks + (j - first)) * 2) * a.dim;
+      store_result_row<float, DP>(part, dk, 1.f, a.dim);
+      store_result_row<float, DP>(part + a.dim, dv, 1.f, a.dim);
+    }
+    return;
+  }
+  if (j >= a.k_len) return;
+  if (g.far_partial && j >= first && j < sink_end) {
+    for (int n = 0; n < g.far_chunks; ++n) {
+      const float* part =
+          g.far_partial + (((((int64_t)b * a.kv_heads + kv) * g.far_chunks + n) * a.sinks + (j - first)) * 2) * a.dim;
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = 32 * dt + result_row(i);
+          if (d < a.dim) {
+            dk[dt][i] += part[d];
+            dv[dt][i] += part[a.dim + d];
+          }
+        }
+    }
+  }
+  const int64_t at = (((int64_t)b * a.k_len + j) * a.kv_heads + kv) * a.dim;
+  store_result_row<T, DP>(static_cast<T*>(g.dk) + at, dk, a.scale, a.dim);
+  store_result_row<T, DP>(static_cast<T*>(g.dv) + at, dv, 1.f, a.dim);
+}
+
+// ---------------------------------------------------------------- host side --
+
+struct BackwardLayout {
+  size_t delta = 0, bias = 0, far = 0, bytes = 0;
+  int64_t bias_parts = 0;
+  int32_t far_chunks = 0;
+  explicit BackwardLayout(const mdl_attention& a) {
+    auto take = [&](size_t n) {
+      const size_t at = bytes;
+      bytes = (bytes + n + 255) & ~size_t(255);
+      return at;
+    };
+    delta = take((size_t)a.batch * a.q_heads * a.q_len * 4);
+    if (a.bias_table) {
+      bias_parts = a.batch * ((a.q_len + kAttnRows - 1) / kAttnRows);
+      bias = take((size_t)bias_parts * a.q_heads * a.num_buckets * 4);
+    }
+    if (a.window > 0 && a.window < a.k_len && a.sinks > 0) {
+      const int64_t sinks = a.sinks < a.k_len ? a.sinks : a.k_len;
+      far_chunks = (int32_t)((a.q_len + kFarRows - 1) / kFarRows);
+      far = take((size_t)a.batch * a.kv_heads * far_chunks * sinks * 2 * a.head_dim * 4);
+    }
+  }
+};
+
+template <typename T, int DP, bool kVec>
+int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
+  using F = Frags<T>;
+  const size_t tiles = (size_t)4 * F::kTile * (DP + F::kPad) * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
+  {
+    const int64_t blocks = (int64_t)((a.q_len + kAttnRows - 1) / kAttnRows) * a.q_heads * a.batch;
+    const size_t lds = tiles + (g.bias_partial ? (size_t)8 * (a.distances + 2 * kSpare) * sizeof(float) : 0);
+    const auto kernel = attention_grad_q_kernel<T, DP, kVec>;
+    if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
+    if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
+    MDL_CHECK_LAUNCH("attention_grad_q_kernel");
+  }
+  const size_t lds = tiles + (size_t)6 * F::kTile * sizeof(float);
+  if (g.far_partial) {
+    const int64_t blocks =
+        (int64_t)((a.sinks + kAttnRows - 1) / kAttnRows) * g.far_chunks * a.kv_heads * a.batch;
+    const auto kernel = attention_grad_kv_kernel<T, DP, kVec, true>;
+    if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
+    if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
+    MDL_CHECK_LAUNCH("attention_grad_kv_kernel");
+  }
+  const int64_t blocks = (int64_t)((a.k_len + kAttnRows - 1) / kAttnRows) * a.kv_heads * a.batch;
+  const auto kernel = attention_grad_kv_kernel<T, DP, kVec, false>;
+  if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
+  MDL_CHECK_LAUNCH("attention_grad_kv_kernel");
+  return MDL_OK;
+}
+
+}  // namespace mdl
+
+using namespace mdl;
+
+extern "C" {
+
+size_t mdl_attention_backward_workspace_bytes(const mdl_attention* a) { return a ? BackwardLayout(*a).bytes : 0; }
+
+int mdl_attention_backward(const mdl_attention* a, const void* prepared, const mdl_attention_grads* grads,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = attention_check(a, "mdl_attention_backward")) return rc;
+  if (!grads) return fail(MDL_ERR_INVALID, "mdl_attention_backward: null pointer");
+  if (a->batch == 0 || a->q_len == 0) return MDL_OK;
+  if (!grads->out || !grads->stats || !grads->grad_out || !grads->grad_q || !grads->grad_k || !grads->grad_v ||
+      (mdl_attention_prepared_bytes(a) && !prepared))
+    return fail(MDL_ERR_INVALID, "mdl_attention_backward: null pointer");
+  if (grads->grad_table && !a->bias_table)
+    return fail(MDL_ERR_INVALID, "mdl_attention_backward: grad_table without a bias_table");
+  const BackwardLayout lay(*a);
+  if (!workspace || workspace_bytes < lay.bytes)
+    return fail(MDL_ERR_WORKSPACE, "mdl_attention_backward: workspace too small");
+  const AttnCall c = attention_call(*a, prepared);
+  char* ws = static_cast<char*>(workspace);
+  GradCall g{};
+  g.out = grads->out;
+  g.stats = reinterpret_cast<const float2*>(grads->stats);
+  g.grad_out = grads->grad_out;
+  g.g_batch = grads->grad_batch; g.g_row = grads->grad_row; g.g_head = grads->grad_head;
+  g.dq = grads->grad_q; g.dk = grads->grad_k; g.dv = grads->grad_v;
+  g.delta = reinterpret_cast<float*>(ws + lay.delta);
+  g.starts = a->bucket_starts;
+  g.buckets = a->num_buckets;
+  g.bias_partial = grads->grad_table ? reinterpret_cast<float*>(ws + lay.bias) : nullptr;
+  g.far_partial = lay.far_chunks ? reinterpret_cast<float*>(ws + lay.far) : nullptr;
+  g.far_chunks = lay.far_chunks;
+  const int64_t e = a->dtype == MDL_BF16 ? 8 : 4;
+  const bool vec = attention_vectors(*a) && reinterpret_cast<uintptr_t>(g.grad_out) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.g_batch % e == 0 && g.g_row % e == 0 &&
+                   g.g_head % e == 0;
+  const hipStream_t s = as_stream(stream);
+  if (int rc = for_attention(*a, vec, [&]<typename T, int DP, bool kVec>() {
+        return launch_backward<T, DP, kVec>(c, g, s);
+      }))
+    return rc;
+  if (grads->grad_table) {
+    const dim3 grid((unsigned)((a->num_buckets + 7) / 8), (unsigned)a->q_heads);
+    if (a->table_dtype == MDL_F32)
+      hipLaunchKernelGGL(bias_partial_sum_kernel<float>, grid, dim3(256), 0, s, g.bias_partial, lay.bias_parts,
+                         a->num_buckets, a->q_heads, static_cast<float*>(grads->grad_table));
+    else
+      hipLaunchKernelGGL(bias_partial_sum_kernel<bf16_t>, grid, dim3(256), 0, s, g.bias_partial, lay.bias_parts,
+                         a->num_buckets, a->q_heads, static_cast<bf16_t*>(grads->grad_table));
+    MDL_CHECK_LAUNCH("bias_partial_sum_kernel");
+  }
+  return MDL_OK;
+}
+
+}  // extern "C"

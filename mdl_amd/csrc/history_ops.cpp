@@ -1,0 +1,260 @@
+// Operators over long histories (namespace mdl_hip), in C++: the window
+// attention with its gradient.  Each operator's ROCm kernel calls the C ABI of
+// libmdl_hip.so on the current HIP stream; CPU and fake kernels are registered
+// by mdl_amd/history.py on these schemas.  The gradient is an autograd node
+// made here, so that a training step's Python is one call.
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <tuple>
+
+#include "../../include/mdl_hip.h"
+#include "torch_ops.h"
+
+namespace mdl_torch {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+at::TensorOptions options_of(const Tensor& t, at::ScalarType type) {
+  return at::TensorOptions().dtype(type).device(t.device());
+}
+
+// The last dimension contiguous (any strides over the others).
+Tensor inner_contiguous(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+void same_device(const Tensor& t, const Tensor& q, const char* what) {
+  TORCH_CHECK_VALUE(t.device() == q.device(), what, " must live on the queries' device");
+}
+
+// ------------------------------------------------------------- attention --
+
+struct AttentionArgs {
+  Tensor q, k, v, mask, table, starts;  // as the kernels read them (held while they run)
+  mdl_attention call{};
+};
+
+void bias_args(const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts, int64_t distances,
+               const Tensor& q, int64_t heads, Tensor& table, Tensor& starts) {
+  TORCH_CHECK_VALUE(bucket_starts.has_value(), "a bias table needs its buckets");
+  TORCH_CHECK_VALUE(bias_table->dim() == 2 && bias_table->size(1) == heads && bias_table->size(0) >= 1,
+                    "bias_table must be [buckets, ", heads, "]");
+  dtype_code(bias_table->scalar_type());
+  same_device(*bias_table, q, "bias_table");
+  same_device(*bucket_starts, q, "bucket_starts");
+  TORCH_CHECK_VALUE(bucket_starts->scalar_type() == at::kInt && bucket_starts->dim() == 1 &&
+                        bucket_starts->is_contiguous() && bucket_starts->size(0) == bias_table->size(0) - 1,
+                    "bucket_starts must be contiguous int32 with one entry fewer than the table has buckets");
+  TORCH_CHECK_VALUE(distances >= 1 && distances <= 2049, "bias buckets must begin at distances up to 2048");
+  table = bias_table->contiguous();
+  starts = *bucket_starts;
+}
+
+AttentionArgs attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
+                             const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts,
+                             int64_t distances, int64_t window, int64_t sinks, double scale) {
+  require_device(q, "attention queries");
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4,
+                    "attention takes q [B, Lq, Hq, D], k and v [B, Lk, Hkv, D]");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(3) == q.size(3),
+                    "attention queries, keys and values are misaligned");
+  TORCH_CHECK_VALUE(q.size(2) > 0 && k.size(2) > 0 && q.size(2) % k.size(2) == 0,
+                    "attention query heads must be a multiple of the key heads");
+  TORCH_CHECK_VALUE(q.size(1) <= k.size(1), "attention queries are the last rows of the keys: more queries than keys");
+  TORCH_CHECK_VALUE(q.size(3) >= 1 && q.size(3) <= 128, "attention head dimension must be 1 to 128");
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                   "attention queries, keys and values must have one dtype");
+  TORCH_CHECK_VALUE(window >= 0, "attention window must be positive");
+  TORCH_CHECK_VALUE(sinks >= 0, "attention sinks must not be negative");
+  TORCH_CHECK_VALUE(scale > 0 && scale < 1e30, "attention scale must be positive");
+  same_device(k, q, "attention keys");
+  same_device(v, q, "attention values");
+  AttentionArgs a;
+  mdl_attention& c = a.call;
+  c.dtype = dtype_code(q.scalar_type());
+  a.q = inner_contiguous(q);
+  a.k = inner_contiguous(k);
+  a.v = inner_contiguous(v);
+  if (mask.has_value()) {
+    TORCH_CHECK_VALUE(mask->dim() == 2 && mask->size(0) == k.size(0) && mask->size(1) == k.size(1),
+                      "attention mask must be [B, Lk]");
+    TORCH_CHECK_TYPE(mask->scalar_type() == at::kBool, "attention mask must be torch.bool");
+    same_device(*mask, q, "attention mask");
+    a.mask = inner_contiguous(*mask);
+    c.mask = static_cast<const uint8_t*>(a.mask.data_ptr());
+    c.mask_row = a.mask.stride(0);
+  }
+  if (bias_table.has_value()) {
+    bias_args(bias_table, bucket_starts, distances, q, q.size(2), a.table, a.starts);
+    c.bias_table = a.table.data_ptr();
+    c.bucket_starts = static_cast<const int32_t*>(a.starts.data_ptr());
+    c.table_dtype = dtype_code(a.table.scalar_type());
+    c.num_buckets = (int32_t)a.table.size(0);
+    c.distances = (int32_t)distances;
+  }
+  c.q = a.q.data_ptr(); c.k = a.k.data_ptr(); c.v = a.v.data_ptr();
+  c.batch = q.size(0); c.q_len = q.size(1); c.k_len = k.size(1);
+  c.q_batch = a.q.stride(0); c.q_row = a.q.stride(1); c.q_head = a.q.stride(2);
+  c.k_batch = a.k.stride(0); c.k_row = a.k.stride(1); c.k_head = a.k.stride(2);
+  c.v_batch = a.v.stride(0); c.v_row = a.v.stride(1); c.v_head = a.v.stride(2);
+  c.window = window;
+  c.sinks = sinks;
+  c.q_heads = (int32_t)q.size(2); c.kv_heads = (int32_t)k.size(2); c.head_dim = (int32_t)q.size(3);
+  c.scale = (float)scale;
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> attention_forward_cuda(
+    const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
+    const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts, int64_t distances,
+    int64_t window, int64_t sinks, double scale, bool need_backward) {
+  const AttentionArgs a =
+      attention_args(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
+  c10::DeviceGuard guard(q.device());
+  void* stream = stream_of(q.device());
+  Tensor out = at::empty(q.sizes(), options_of(q, q.scalar_type()));
+  Tensor stats = need_backward ? at::empty({q.size(0), q.size(2), q.size(1), 2}, options_of(q, at::kFloat))
+                               : at::empty({0}, options_of(q, at::kFloat));
+  const size_t bytes = mdl_attention_prepared_bytes(&a.call);
+  Tensor prepared = at::empty({(int64_t)bytes}, options_of(q, at::kByte));
+  check(mdl_attention_prepare(&a.call, prepared.data_ptr(), bytes, stream), "mdl_attention_prepare");
+  check(mdl_attention_forward(&a.call, prepared.data_ptr(), out.data_ptr(),
+                              need_backward ? static_cast<float*>(stats.data_ptr()) : nullptr, stream),
+        "mdl_attention_forward");
+  return {out, stats, prepared};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
+    const Tensor& grad_out, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
+    const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts, int64_t distances,
+    int64_t window, int64_t sinks, double scale, const Tensor& out, const Tensor& stats, const Tensor& prepared,
+    bool need_table) {
+  const AttentionArgs a =
+      attention_args(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
+  TORCH_CHECK_VALUE(grad_out.sizes() == q.sizes() && out.sizes() == q.sizes() && out.is_contiguous(),
+                    "attention gradient and output must have the queries' shape");
+  TORCH_CHECK_TYPE(grad_out.scalar_type() == q.scalar_type() && out.scalar_type() == q.scalar_type(),
+                   "attention gradient and output must have the queries' dtype");
+  TORCH_CHECK_VALUE(stats.numel() == 2 * q.size(0) * q.size(1) * q.size(2) && stats.scalar_type() == at::kFloat &&
+                        stats.is_contiguous() && (size_t)prepared.numel() >= mdl_attention_prepared_bytes(&a.call),
+                    "attention backward needs the forward's statistics");
+  same_device(grad_out, q, "attention gradient");
+  c10::DeviceGuard guard(q.device());
+  const Tensor go = inner_contiguous(grad_out);
+  Tensor dq = at::empty(q.sizes(), options_of(q, q.scalar_type()));
+  Tensor dk = at::empty(k.sizes(), options_of(k, k.scalar_type()));
+  Tensor dv = at::empty(v.sizes(), options_of(v, v.scalar_type()));
+  need_table = need_table && bias_table.has_value();
+  Tensor dtable = need_table ? at::empty(bias_table->sizes(), options_of(q, bias_table->scalar_type()))
+                             : at::empty({0}, options_of(q, q.scalar_type()));
+  if (q.numel() == 0) {
+    dk.zero_();
+    dv.zero_();
+    dtable.zero_();
+    return {dq, dk, dv, dtable};
+  }
+  mdl_attention_grads g{};
+  g.out = out.data_ptr();
+  g.stats = static_cast<const float*>(stats.data_ptr());
+  g.grad_out = go.data_ptr();
+  g.grad_batch = go.stride(0); g.grad_row = go.stride(1); g.grad_head = go.stride(2);
+  g.grad_q = dq.data_ptr(); g.grad_k = dk.data_ptr(); g.grad_v = dv.data_ptr();
+  g.grad_table = need_table ? dtable.data_ptr() : nullptr;
+  const size_t bytes = mdl_attention_backward_workspace_bytes(&a.call);
+  Tensor ws = workspace(bytes, q.device());
+  check(mdl_attention_backward(&a.call, prepared.data_ptr(), &g, ws.data_ptr(), bytes, stream_of(q.device())),
+        "mdl_attention_backward");
+  return {dq, dk, dv, dtable};
+}
+
+std::tuple<Tensor, Tensor, Tensor> call_attention_forward(
+    const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
+    const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts, int64_t distances,
+    int64_t window, int64_t sinks, double scale, bool need_backward) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("mdl_hip::history_attention_forward", "")
+                             .typed<decltype(attention_forward_cuda)>();
+  return op.call(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale, need_backward);
+}
+
+Tensor history_attention_plain(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
+                               const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts,
+                               int64_t distances, int64_t window, int64_t sinks, double scale) {
+  return std::get<0>(call_attention_forward(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale,
+                                            false));
+}
+
+std::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const std::optional<Tensor>& mask, const std::optional<Tensor>& bias_table,
+                        const std::optional<Tensor>& bucket_starts, int64_t distances, int64_t window, int64_t sinks,
+                        double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, stats, prepared] =
+        call_attention_forward(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale, true);
+    ctx->save_for_backward({q, k, v, mask.value_or(Tensor()), bias_table.value_or(Tensor()),
+                            bucket_starts.value_or(Tensor()), out, stats, prepared});
+    ctx->saved_data["distances"] = distances;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("mdl_hip::history_attention_backward", "")
+                               .typed<decltype(attention_backward_cuda)>();
+    auto [dq, dk, dv, dtable] =
+        op.call(grads[0], s[0], s[1], s[2], optional_of(s[3]), optional_of(s[4]), optional_of(s[5]),
+                ctx->saved_data["distances"].toInt(), ctx->saved_data["window"].toInt(),
+                ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble(), s[6], s[7], s[8],
+                s[4].defined() && ctx->needs_input_grad(4));
+    const Tensor none;
+    return {dq, dk, dv, none, s[4].defined() && ctx->needs_input_grad(4) ? dtable : none, none, none, none, none, none};
+  }
+};
+
+Tensor history_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
+                                  const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts,
+                                  int64_t distances, int64_t window, int64_t sinks, double scale) {
+  const bool need = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                                   (bias_table.has_value() && bias_table->requires_grad()));
+  if (need) return HistoryAttention::apply(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return history_attention_plain(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
+}
+
+}  // namespace
+}  // namespace mdl_torch
+
+TORCH_LIBRARY_FRAGMENT(mdl_hip, m) {
+  m.def("history_attention(Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor? bias_table, Tensor? bucket_starts, "
+        "int distances, int window, int sinks, float scale) -> Tensor");
+  m.def("history_attention_forward(Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor? bias_table, "
+        "Tensor? bucket_starts, int distances, int window, int sinks, float scale, bool need_backward) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("history_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor? bias_table, "
+        "Tensor? bucket_starts, int distances, int window, int sinks, float scale, Tensor out, Tensor stats, "
+        "Tensor prepared, bool need_table) -> (Tensor, Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(mdl_hip, CUDA, m) {
+  using namespace mdl_torch;
+  m.impl("history_attention_forward", &attention_forward_cuda);
+  m.impl("history_attention_backward", &attention_backward_cuda);
+}
+
+TORCH_LIBRARY_IMPL(mdl_hip, CompositeExplicitAutograd, m) {
+  m.impl("history_attention", &mdl_torch::history_attention_plain);
+}
+
+TORCH_LIBRARY_IMPL(mdl_hip, Autograd, m) { m.impl("history_attention", &mdl_torch::history_attention_autograd); }

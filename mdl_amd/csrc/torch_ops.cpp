@@ -45,6 +45,7 @@
 #include <vector>
 
 #include "../../include/mdl_hip.h"
+#include "torch_ops.h"
 
 namespace mdl_torch {
 
