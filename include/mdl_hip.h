@@ -722,6 +722,49 @@ size_t mdl_attention_backward_workspace_bytes(const mdl_attention* call);
 int mdl_attention_backward(const mdl_attention* call, const void* prepared, const mdl_attention_grads* grads,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * One new token a row over a cache.  Row b's token stands at position n =
+ * positions[b]; position p is held in slot p for p < sinks and in slot
+ * sinks + (p - sinks) % (capacity - sinks) otherwise, so a cache of the
+ * window and the first tokens alone turns as a ring and a longer one is a
+ * plain array.  The step stores k and v [batch, kv_heads, head_dim] in the
+ * token's slot and answers q [batch, q_heads, head_dim] over the positions
+ * p <= n with n - p < window or p < sinks (window <= 0: all that the cache
+ * holds).  Slots of other positions are not read.  A negative position
+ * stores nothing and is answered with zeros.  Scores and bias as in
+ * mdl_attention.  out: [batch, q_heads, head_dim] contiguous.
+ */
+typedef struct mdl_attention_step {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* cache_k;                 /* [batch, capacity, kv_heads, head_dim], head_dim contiguous */
+  void* cache_v;
+  const int64_t* positions;      /* [batch] */
+  const void* bias_table;
+  const int32_t* bucket_starts;
+  int64_t batch, capacity;
+  int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head;  /* element strides */
+  int64_t ck_batch, ck_slot, ck_head, cv_batch, cv_slot, cv_head;
+  int64_t window;                /* at most capacity - sinks */
+  int64_t sinks;
+  int32_t q_heads, kv_heads, head_dim, dtype;
+  int32_t table_dtype, num_buckets, distances;
+  float scale;
+} mdl_attention_step;
+
+size_t mdl_attention_step_workspace_bytes(const mdl_attention_step* step);
+int mdl_attention_step_forward(const mdl_attention_step* step, void* out, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* The cache's prompt form: k and v [batch, len, kv_heads, head_dim] (batch
+ * and head strides of the descriptor, row strides k_row and v_row) hold each
+ * row's positions 0 .. lengths[b] - 1 in their first rows, or their last ones
+ * with right_aligned; those that no later position of the same slot replaces
+ * are stored.  q, positions and the bias of the descriptor are not used. */
+int mdl_attention_cache_write(const mdl_attention_step* step, int64_t len, int64_t k_row, int64_t v_row,
+                              const int64_t* lengths, int32_t right_aligned, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,7 +114,17 @@ ATTENTION_GRADS_DTYPE = np.dtype(
     + [(name, "<i8") for name in ("grad_batch", "grad_row", "grad_head")]
     + [(name, "<u8") for name in ("grad_q", "grad_k", "grad_v", "grad_table")]
 )
+ATTENTION_STEP_DTYPE = np.dtype(
+    [(name, "<u8") for name in ("q", "k", "v", "cache_k", "cache_v", "positions", "bias_table", "bucket_starts")]
+    + [(name, "<i8") for name in (
+        "batch", "capacity", "q_batch", "q_head", "k_batch", "k_head", "v_batch", "v_head", "ck_batch", "ck_slot",
+        "ck_head", "cv_batch", "cv_slot", "cv_head", "window", "sinks")]
+    + [(name, "<i4") for name in (
+        "q_heads", "kv_heads", "head_dim", "dtype", "table_dtype", "num_buckets", "distances")]
+    + [("scale", "<f4")]
+)
 assert ATTENTION_DTYPE.itemsize == 200
+assert ATTENTION_STEP_DTYPE.itemsize == 224
 assert ATTENTION_GRADS_DTYPE.itemsize == 80
 
 _P = ctypes.c_void_p
@@ -196,6 +206,9 @@ SIGNATURES: dict[str, tuple] = {
     "mdl_attention_forward": (_I32, [_P, _P, _P, _P, _P]),
     "mdl_attention_backward_workspace_bytes": (_SZ, [_P]),
     "mdl_attention_backward": (_I32, [_P, _P, _P, _P, _SZ, _P]),
+    "mdl_attention_step_workspace_bytes": (_SZ, [_P]),
+    "mdl_attention_step_forward": (_I32, [_P, _P, _P, _SZ, _P]),
+    "mdl_attention_cache_write": (_I32, [_P, _I64, _I64, _I64, _P, _I32, _P]),
     "mdl_rowwise_adagrad": (
         _I32,
         [_P, _I32, _I64, _I32, _I64, _P, _P, _I64, _P, _I32, _I64, _F, _F, _P, _P],

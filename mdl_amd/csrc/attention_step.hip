@@ -1,0 +1,532 @@
+// Attention of one new token a row over a cache of keys and values, and the
+// cache's prompt form.
+//
+// A step reads every visible key and value once and does two multiply-adds
+// per element and query head that shares it: bytes bound it (the heads that
+// share a key head are answered together, up to 8 of them), so it runs on the
+// vector units.  A lane group covers one cached row in 16-byte pieces and
+// walks every (groups of the block)-th row with its own running maximum and
+// sum; groups, then waves, then blocks are joined at the end.  Few rows with
+// long caches are cut into parts over several blocks, joined by a second
+// launch.
+#include "attention.cuh"
+
+namespace mdl {
+
+constexpr int kStepThreads = 256;
+constexpr int kStepUnroll = 4;     // rows in flight per lane group
+constexpr int kStepBlocks = 1024;  // blocks wanted before a row's walk is no longer cut
+constexpr int kStepMinRows = 512;  // cached rows of a part at least
+
+struct StepCall {
+  const void *q, *k, *v;
+  void *cache_k, *cache_v;
+  const int64_t* positions;
+  const void* table;
+  const int32_t* starts;
+  float* part;  // [B * Hq, parts, 2 + dim]: maximum, sum, sums of values; NULL with one part
+  int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head;
+  int64_t ck_batch, ck_slot, ck_head, cv_batch, cv_slot, cv_head;
+  int64_t window, sinks, ring;  // window <= ring
+  int32_t batch, q_heads, kv_heads, dim, parts, buckets, distances, table_f32;
+  float c2;  // scale * log2(e)
+};
+
+// The cached rows a token at position n sees, in order: the first tokens,
+// then those of the window; the last one is the token itself.
+struct StepRows {
+  int64_t sinks, from, base, ring, at_sinks, count;
+  __device__ __forceinline__ StepRows(const StepCall& a, int64_t n) {
+    sinks = a.sinks < n + 1 ? a.sinks : n + 1;
+    from = n - a.window + 1;
+    if (from < a.sinks) from = a.sinks;
+    ring = a.ring;
+    at_sinks = a.sinks;
+    base = from <= n ? (from - a.sinks) % ring : 0;
+    count = sinks + (from <= n ? n - from + 1 : 0);
+  }
+  __device__ __forceinline__ int64_t position(int64_t i) const { return i < sinks ? i : from + (i - sinks); }
+  __device__ __forceinline__ int64_t slot(int64_t i) const {
+    if (i < sinks) return i;
+    int64_t x = base + (i - sinks);  // the window is no longer than the ring: one turn at most
+    if (x >= ring) x -= ring;
+    return at_sinks + x;
+  }
+  // rows of one part, whole parts of at least kStepMinRows
+  __device__ __forceinline__ int64_t per_part(int parts) const {
+    const int64_t per = (count + parts - 1) / parts;
+    return per > kStepMinRows ? per : kStepMinRows;
+  }
+};
+
+// Sum over aligned groups of N lanes, in every lane.
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+  auto dpp = [&](auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if constexpr (N >= 2) v += dpp(std::integral_constant<int, 0xB1>{});   // quad: 1 0 3 2
+  if constexpr (N >= 4) v += dpp(std::integral_constant<int, 0x4E>{});   // quad: 2 3 0 1
+  if constexpr (N >= 8) v += dpp(std::integral_constant<int, 0x141>{});  // mirror of 8
+  if constexpr (N >= 16) v += dpp(std::integral_constant<int, 0x140>{}); // mirror of 16
+  if constexpr (N >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float element(const typename Frags<T>::Frag& f, int i) {
+  return (float)f[i];
+}
+
+// One head group's running softmax over its lanes' values.
+template <int G, int E>
+struct StepState {
+  float m[G], l[G], acc[G][E];
+  __device__ __forceinline__ StepState() {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      m[g] = kNoScore;
+      l[g] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[g][e] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void raise(int g, float top) {
+    const float shrink = exp2_fast(m[g] - top);
+    m[g] = top;
+    l[g] *= shrink;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[g][e] *= shrink;
+  }
+  __device__ __forceinline__ void join_lanes(int distance) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float m2 = __shfl_xor(m[g], distance);
+      raise(g, fmaxf(m[g], m2));
+      l[g] += __shfl_xor(l[g], distance);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[g][e] += __shfl_xor(acc[g][e], distance);
+    }
+  }
+};
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void store_piece(T* row, int d, int D, const float* v) {
+  constexpr int E = Frags<T>::kElems;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (kVec ? d < D : d + i < D) {
+      if constexpr (sizeof(T) == 2) *(gptr<__bf16>)(row + d + i) = (__bf16)v[i];
+      else *to_global(row + d + i) = v[i];
+    }
+}
+
+template <typename T, int L, int G, bool kVec>
+__global__ __launch_bounds__(kStepThreads) void attention_step_kernel(StepCall a, T* out) {
+  using F = Frags<T>;
+  constexpr int E = F::kElems, kGroups = kWave / L, kWaves = kStepThreads / kWave;
+  constexpr int kPass = kGroups * kStepUnroll;  // rows of a wave's iteration
+  extern __shared__ __align__(16) char smem[];
+  float* lds_table = reinterpret_cast<float*>(smem);           // [buckets][G] bias in powers of two
+  uint16_t* lds_bucket = reinterpret_cast<uint16_t*>(lds_table + a.buckets * G);  // [distances]
+  __shared__ float lds_join[kWaves][L][G][E + 2];
+
+  const int share = a.q_heads / a.kv_heads, groups = (share + G - 1) / G;
+  int64_t id = blockIdx.x;
+  const int part = (int)(id % a.parts);
+  id /= a.parts;
+  const int hg = (int)(id % groups);
+  id /= groups;
+  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
+  const int head0 = kv * share + hg * G, heads = share - hg * G < G ? share - hg * G : G;
+  const int wave = threadIdx.x / kWave, sub = lane_id() % L, group = lane_id() / L;
+  const int d = sub * E;
+  T* out_row = out + ((int64_t)b * a.q_heads + head0) * a.dim;
+
+  const int64_t n = a.positions[b];
+  if (n < 0) {  // no such position: nothing stored, zeros answered
+    if (part == 0)
+      for (int i = threadIdx.x; i < heads * a.dim; i += kStepThreads) out_row[i] = T(0);
+    return;
+  }
+  const StepRows rows(a, n);
+  const int64_t per = rows.per_part(a.parts);
+  const int64_t lo = part * per, hi = lo + per < rows.count ? lo + per : rows.count;
+  if (lo >= hi) return;
+
+  if (a.table) {
+    for (int i = threadIdx.x; i < a.buckets * G; i += kStepThreads) {
+      const int g = i % G;
+      float v = 0.f;
+      if (g < heads) {
+        const int64_t at = (int64_t)(i / G) * a.q_heads + head0 + g;
+        v = a.table_f32 ? static_cast<const float*>(a.table)[at]
+                        : bf16_to_f32(static_cast<const bf16_t*>(a.table)[at]);
+        const bool finite = __builtin_isfinite(v);
+        v *= 1.4426950408889634f;
+        if (finite) v = fminf(fmaxf(v, kLowScore), -kLowScore);
+      }
+      lds_table[i] = v;
+    }
+    // bucket by bucket: every distance from its start to the next one's
+    for (int k = wave; k < a.buckets; k += kWaves) {
+      const int from = k == 0 ? 0 : a.starts[k - 1];
+      const int to = k == a.buckets - 1 ? a.distances : a.starts[k];
+      for (int x = from + lane_id(); x < to; x += kWave) lds_bucket[x] = (uint16_t)k;
+    }
+    __syncthreads();
+  }
+
+  const T* new_k = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
+  const T* new_v = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
+  T* cache_k = static_cast<T*>(a.cache_k) + b * a.ck_batch + kv * a.ck_head;
+  T* cache_v = static_cast<T*>(a.cache_v) + b * a.cv_batch + kv * a.cv_head;
+
+  float q[G][E];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    typename F::Frag f = {};
+    if (g < heads)
+      f = load_row<T, kVec>(static_cast<const T*>(a.q) + b * a.q_batch + (int64_t)(head0 + g) * a.q_head, d, a.dim);
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[g][e] = element<T>(f, e) * a.c2;
+  }
+
+  StepState<G, E> st;
+  const int64_t last = rows.count - 1;
+  for (int64_t i0 = lo + wave * kPass; i0 < hi; i0 += kWaves * kPass) {
+    typename F::Frag kf[kStepUnroll], vf[kStepUnroll];
+#pragma unroll
+    for (int u = 0; u < kStepUnroll; ++u) {
+      const int64_t i = i0 + u * kGroups + group;
+      kf[u] = {};
+      vf[u] = {};
+      if (i < hi) {
+        const int64_t slot = rows.slot(i);
+        kf[u] = load_row<T, kVec>(i == last ? new_k : cache_k + slot * a.ck_slot, d, a.dim);
+        vf[u] = load_row<T, kVec>(i == last ? new_v : cache_v + slot * a.cv_slot, d, a.dim);
+      }
+    }
+    float s[kStepUnroll][G];
+#pragma unroll
+    for (int u = 0; u < kStepUnroll; ++u) {
+      const int64_t i = i0 + u * kGroups + group;
+      const float* bias = nullptr;
+      if (a.table && i < hi) {
+        const int64_t x = n - rows.position(i);
+        bias = lds_table + (x < a.distances ? lds_bucket[x] : a.buckets - 1) * G;
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) t = __builtin_fmaf(q[g][e], element<T>(kf[u], e), t);
+        t = group_sum<L>(t);
+        if (bias) t += bias[g];
+        s[u][g] = i < hi ? t : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float top = s[0][g];
+#pragma unroll
+      for (int u = 1; u < kStepUnroll; ++u) top = fmaxf(top, s[u][g]);
+      if (__any(top > st.m[g] + 8.f)) st.raise(g, fmaxf(st.m[g], top));
+#pragma unroll
+      for (int u = 0; u < kStepUnroll; ++u) {
+        const float p = exp2_fast(s[u][g] - st.m[g]);
+        st.l[g] += p;
+#pragma unroll
+        for (int e = 0; e < E; ++e) st.acc[g][e] = __builtin_fmaf(p, element<T>(vf[u], e), st.acc[g][e]);
+      }
+    }
+  }
+  // the new token's row takes its slot (this step reads it from the input)
+  if (hi == rows.count && hg == 0 && wave == kWaves - 1 && group == 0) {
+    const int64_t slot = rows.slot(last);
+    const typename F::Frag kf = load_row<T, kVec>(new_k, d, a.dim), vf = load_row<T, kVec>(new_v, d, a.dim);
+    float kx[E], vx[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      kx[e] = element<T>(kf, e);
+      vx[e] = element<T>(vf, e);
+    }
+    store_piece<T, kVec>(cache_k + slot * a.ck_slot, d, a.dim, kx);
+    store_piece<T, kVec>(cache_v + slot * a.cv_slot, d, a.dim, vx);
+  }
+
+#pragma unroll
+  for (int x = L; x < kWave; x <<= 1) st.join_lanes(x);
+  if (group == 0)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      lds_join[wave][sub][g][0] = st.m[g];
+      lds_join[wave][sub][g][1] = st.l[g];
+#pragma unroll
+      for (int e = 0; e < E; ++e) lds_join[wave][sub][g][2 + e] = st.acc[g][e];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < L * heads; i += kStepThreads) {
+    const int g = i / L, at = i % L;
+    float m = lds_join[0][at][g][0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds_join[w][at][g][0]);
+    float l = 0.f, v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_fast(lds_join[w][at][g][0] - m);
+      l += lds_join[w][at][g][1] * f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] += lds_join[w][at][g][2 + e] * f;
+    }
+    if (a.parts == 1) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] *= inv;
+      store_piece<T, kVec>(out_row + (int64_t)g * a.dim, at * E, a.dim, v);
+    } else {
+      float* p = a.part + (((int64_t)b * a.q_heads + head0 + g) * a.parts + part) * (2 + a.dim);
+      if (at == 0) {
+        p[0] = m;
+        p[1] = l;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at * E + e < a.dim) p[2 + at * E + e] = v[e];
+    }
+  }
+}
+
+// Joins the parts of a row's walk: one wave per row and head.
+template <typename T>
+__global__ __launch_bounds__(kStepThreads) void attention_step_join_kernel(StepCall a, T* out) {
+  const int64_t at = (int64_t)blockIdx.x * (kStepThreads / kWave) + threadIdx.x / kWave;
+  if (at >= (int64_t)a.batch * a.q_heads) return;
+  const int64_t n = a.positions[at / a.q_heads];
+  if (n < 0) return;
+  const StepRows rows(a, n);
+  const int64_t per = rows.per_part(a.parts);
+  const int parts = (int)((rows.count + per - 1) / per);
+  const float* p = a.part + at * a.parts * (2 + a.dim);
+  float m = kNoScore;
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, p[(int64_t)i * (2 + a.dim)]);
+  float l = 0.f, v[2] = {0.f, 0.f};
+  for (int i = 0; i < parts; ++i) {
+    const float* x = p + (int64_t)i * (2 + a.dim);
+    const float f = exp2_fast(x[0] - m);
+    l += x[1] * f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (lane_id() + kWave * c < a.dim) v[c] += x[2 + lane_id() + kWave * c] * f;
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (lane_id() + kWave * c < a.dim) {
+      const float o = v[c] * inv;
+      if constexpr (sizeof(T) == 2) out[at * a.dim + lane_id() + kWave * c] = f32_to_bf16(o);
+      else out[at * a.dim + lane_id() + kWave * c] = o;
+    }
+}
+
+// The prompt form: rows of k and v at positions 0 .. length - 1 take their
+// slots, those that a later one of the same slot replaces left out.  One
+// block per (batch row, 64 rows); a thread moves elements of one row.
+template <typename T>
+__global__ __launch_bounds__(256) void cache_write_kernel(StepCall a, int64_t len, const int64_t* lengths,
+                                                           int32_t right_aligned) {
+  const int b = blockIdx.y;
+  int64_t n = lengths[b];
+  if (n > len) n = len;
+  const int64_t shift = right_aligned ? len - n : 0;
+  const int width = a.kv_heads * a.dim;
+  const int64_t r0 = (int64_t)blockIdx.x * 64;
+  for (int64_t i = threadIdx.x; i < 64 * (int64_t)width; i += 256) {
+    const int64_t r = r0 + i / width, p = r - shift;
+    const int c = (int)(i % width), kv = c / a.dim, d = c % a.dim;
+    if (r >= len || p < 0 || p >= n) continue;
+    if (p >= a.sinks && p < n - a.ring) continue;
+    const int64_t slot = p < a.sinks ? p : a.sinks + (p - a.sinks) % a.ring;
+    static_cast<T*>(a.cache_k)[b * a.ck_batch + slot * a.ck_slot + kv * a.ck_head + d] =
+        static_cast<const T*>(a.k)[b * a.k_batch + r * a.q_batch + kv * a.k_head + d];
+    static_cast<T*>(a.cache_v)[b * a.cv_batch + slot * a.cv_slot + kv * a.cv_head + d] =
+        static_cast<const T*>(a.v)[b * a.v_batch + r * a.q_head + kv * a.v_head + d];
+  }
+}
+
+// ---------------------------------------------------------------- host side --
+
+int heads_together(int share) { return share >= 5 ? 8 : (share >= 3 ? 4 : share); }
+
+// Blocks that share a row's walk: as many as fill the card, each with
+// kStepMinRows cached rows at least.
+int step_parts(const mdl_attention_step& a) {
+  const int share = a.q_heads / a.kv_heads, g = heads_together(share);
+  const int64_t units = a.batch * a.kv_heads * ((share + g - 1) / g);
+  const int64_t most = a.window > 0 && a.window + a.sinks < a.capacity ? a.window + a.sinks : a.capacity;
+  int64_t parts = (kStepBlocks + units - 1) / (units > 0 ? units : 1);
+  const int64_t cap = (most + kStepMinRows - 1) / kStepMinRows;
+  if (parts > cap) parts = cap;
+  return parts < 1 ? 1 : (int)parts;
+}
+
+int step_check(const mdl_attention_step* a, const char* what) {
+  const std::string w(what);
+  if (!a) return fail(MDL_ERR_INVALID, w + ": null descriptor");
+  if (a->batch < 0) return fail(MDL_ERR_INVALID, w + ": negative batch");
+  if (a->sinks < 0 || a->capacity <= a->sinks)
+    return fail(MDL_ERR_INVALID, w + ": the capacity must exceed the first tokens kept");
+  if (a->window > 0 && a->window > a->capacity - a->sinks)
+    return fail(MDL_ERR_INVALID, w + ": the window must fit the capacity beside the first tokens");
+  if (a->q_heads <= 0 || a->kv_heads <= 0 || a->q_heads % a->kv_heads)
+    return fail(MDL_ERR_INVALID, w + ": q_heads must be a positive multiple of kv_heads");
+  if (a->head_dim <= 0 || a->head_dim > 128) return fail(MDL_ERR_UNSUPPORTED, w + ": head_dim must be 1..128");
+  if (a->dtype != MDL_F32 && a->dtype != MDL_BF16) return fail(MDL_ERR_INVALID, w + ": dtype");
+  if (a->bias_table) {
+    if (a->table_dtype != MDL_F32 && a->table_dtype != MDL_BF16) return fail(MDL_ERR_INVALID, w + ": table_dtype");
+    if (a->num_buckets < 1 || (a->num_buckets > 1 && !a->bucket_starts) || a->distances < 1)
+      return fail(MDL_ERR_INVALID, w + ": bias buckets");
+    if (a->distances > kMaxDistances || a->num_buckets > 1024)
+      return fail(MDL_ERR_UNSUPPORTED, w + ": bias buckets must begin at distances up to 2048, at most 1024 of them");
+  }
+  if (a->batch > 0 && (!a->k || !a->v || !a->cache_k || !a->cache_v || !a->positions))
+    return fail(MDL_ERR_INVALID, w + ": null pointer");
+  return MDL_OK;
+}
+
+StepCall step_call(const mdl_attention_step& a) {
+  StepCall c{};
+  c.q = a.q; c.k = a.k; c.v = a.v;
+  c.cache_k = a.cache_k; c.cache_v = a.cache_v;
+  c.positions = a.positions;
+  c.table = a.bias_table;
+  c.starts = a.bucket_starts;
+  c.q_batch = a.q_batch; c.q_head = a.q_head;
+  c.k_batch = a.k_batch; c.k_head = a.k_head;
+  c.v_batch = a.v_batch; c.v_head = a.v_head;
+  c.ck_batch = a.ck_batch; c.ck_slot = a.ck_slot; c.ck_head = a.ck_head;
+  c.cv_batch = a.cv_batch; c.cv_slot = a.cv_slot; c.cv_head = a.cv_head;
+  c.sinks = a.sinks;
+  c.ring = a.capacity - a.sinks;
+  c.window = a.window > 0 ? a.window : c.ring;
+  c.batch = (int32_t)a.batch; c.q_heads = a.q_heads; c.kv_heads = a.kv_heads; c.dim = a.head_dim;
+  c.buckets = a.bias_table ? a.num_buckets : 0;
+  c.distances = a.bias_table ? a.distances : 0;
+  c.table_f32 = a.table_dtype == MDL_F32;
+  c.c2 = (float)((double)a.scale * 1.4426950408889634);
+  return c;
+}
+
+bool step_vectors(const mdl_attention_step& a) {
+  const int64_t e = a.dtype == MDL_BF16 ? 8 : 4;
+  auto whole = [&](const void* p, int64_t x, int64_t y, int64_t z) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && x % e == 0 && y % e == 0 && z % e == 0;
+  };
+  return a.head_dim % e == 0 && whole(a.q, a.q_batch, a.q_head, 0) && whole(a.k, a.k_batch, a.k_head, 0) &&
+         whole(a.v, a.v_batch, a.v_head, 0) && whole(a.cache_k, a.ck_batch, a.ck_slot, a.ck_head) &&
+         whole(a.cache_v, a.cv_batch, a.cv_slot, a.cv_head);
+}
+
+template <typename T, int L, int G, bool kVec>
+int launch_step(const StepCall& c, void* out, hipStream_t s) {
+  const int share = c.q_heads / c.kv_heads;
+  const int64_t blocks = (int64_t)c.batch * c.kv_heads * ((share + G - 1) / G) * c.parts;
+  if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_step: too many rows");
+  const size_t lds = ((size_t)c.buckets * G * 4 + (size_t)c.distances * 2 + 15) & ~size_t(15);
+  const auto kernel = attention_step_kernel<T, L, G, kVec>;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kStepThreads), lds, s, c, static_cast<T*>(out));
+  MDL_CHECK_LAUNCH("attention_step_kernel");
+  if (c.parts > 1) {
+    const int64_t joins = ((int64_t)c.batch * c.q_heads + kStepThreads / kWave - 1) / (kStepThreads / kWave);
+    hipLaunchKernelGGL(attention_step_join_kernel<T>, dim3((unsigned)joins), dim3(kStepThreads), 0, s, c,
+                       static_cast<T*>(out));
+    MDL_CHECK_LAUNCH("attention_step_join_kernel");
+  }
+  return MDL_OK;
+}
+
+template <typename T, int L, bool kVec>
+int launch_step_heads(const StepCall& c, void* out, hipStream_t s) {
+  switch (heads_together(c.q_heads / c.kv_heads)) {
+    case 1: return launch_step<T, L, 1, kVec>(c, out, s);
+    case 2: return launch_step<T, L, 2, kVec>(c, out, s);
+    case 4: return launch_step<T, L, 4, kVec>(c, out, s);
+    default: return launch_step<T, L, 8, kVec>(c, out, s);
+  }
+}
+
+// Lanes per cached row: 16-byte pieces, rounded up to a power of two (4 to 32).
+template <typename T, bool kVec>
+int launch_step_lanes(const StepCall& c, void* out, hipStream_t s) {
+  const int pieces = (c.dim + Frags<T>::kElems - 1) / Frags<T>::kElems;
+  if (pieces <= 4) return launch_step_heads<T, 4, kVec>(c, out, s);
+  if (pieces <= 8) return launch_step_heads<T, 8, kVec>(c, out, s);
+  if (pieces <= 16) return launch_step_heads<T, 16, kVec>(c, out, s);
+  if constexpr (sizeof(T) == 4) return launch_step_heads<T, 32, kVec>(c, out, s);
+  return MDL_ERR_UNSUPPORTED;
+}
+
+}  // namespace mdl
+
+using namespace mdl;
+
+extern "C" {
+
+size_t mdl_attention_step_workspace_bytes(const mdl_attention_step* a) {
+  if (!a || step_check(a, "mdl_attention_step")) return 0;
+  const int parts = step_parts(*a);
+  return parts == 1 ? 0 : (size_t)a->batch * a->q_heads * parts * (2 + a->head_dim) * sizeof(float);
+}
+
+int mdl_attention_step_forward(const mdl_attention_step* a, void* out, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  if (int rc = step_check(a, "mdl_attention_step_forward")) return rc;
+  if (!(a->scale > 0.f) || !(a->scale < INFINITY))
+    return fail(MDL_ERR_INVALID, "mdl_attention_step_forward: scale must be positive");
+  if (a->batch == 0) return MDL_OK;
+  if (a->batch > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_step_forward: too many rows");
+  if (!a->q || !out) return fail(MDL_ERR_INVALID, "mdl_attention_step_forward: null pointer");
+  const size_t need = mdl_attention_step_workspace_bytes(a);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(MDL_ERR_WORKSPACE, "mdl_attention_step_forward: workspace too small");
+  StepCall c = step_call(*a);
+  c.parts = step_parts(*a);
+  c.part = static_cast<float*>(workspace);
+  const hipStream_t s = as_stream(stream);
+  if (a->dtype == MDL_BF16)
+    return step_vectors(*a) ? launch_step_lanes<bf16_t, true>(c, out, s) : launch_step_lanes<bf16_t, false>(c, out, s);
+  return step_vectors(*a) ? launch_step_lanes<float, true>(c, out, s) : launch_step_lanes<float, false>(c, out, s);
+}
+
+int mdl_attention_cache_write(const mdl_attention_step* a, int64_t len, int64_t k_row, int64_t v_row,
+                              const int64_t* lengths, int32_t right_aligned, void* stream) {
+  if (!a || !lengths) return fail(MDL_ERR_INVALID, "mdl_attention_cache_write: null pointer");
+  mdl_attention_step with = *a;
+  with.positions = lengths;
+  with.bias_table = nullptr;
+  if (int rc = step_check(&with, "mdl_attention_cache_write")) return rc;
+  if (len < 0) return fail(MDL_ERR_INVALID, "mdl_attention_cache_write: negative length");
+  if (a->batch == 0 || len == 0) return MDL_OK;
+  if (a->batch > 65535 || (len + 63) / 64 > 0x7fffffff)
+    return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_cache_write: too many rows");
+  StepCall c = step_call(with);
+  c.q_batch = k_row;  // the prompt's row strides
+  c.q_head = v_row;
+  const dim3 grid((unsigned)((len + 63) / 64), (unsigned)a->batch);
+  if (a->dtype == MDL_BF16)
+    hipLaunchKernelGGL(cache_write_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream), c, len, lengths,
+                       right_aligned);
+  else
+    hipLaunchKernelGGL(cache_write_kernel<float>, grid, dim3(256), 0, as_stream(stream), c, len, lengths,
+                       right_aligned);
+  MDL_CHECK_LAUNCH("cache_write_kernel");
+  return MDL_OK;
+}
+
+}  // extern "C"

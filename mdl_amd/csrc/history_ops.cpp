@@ -233,6 +233,110 @@ Tensor history_attention_autograd(const Tensor& q, const Tensor& k, const Tensor
   return history_attention_plain(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
 }
 
+// ------------------------------------------------------ single new tokens --
+
+// cache [B, capacity, Hkv, D]: the descriptor's cache and prompt or token sides.
+mdl_attention_step cache_args(const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v,
+                              int64_t sinks) {
+  require_device(cache_k, "history cache");
+  TORCH_CHECK_VALUE(cache_k.dim() == 4 && cache_k.sizes() == cache_v.sizes(),
+                    "history cache keys and values must be [B, capacity, Hkv, D]");
+  TORCH_CHECK_VALUE(cache_k.stride(3) == 1 && cache_v.stride(3) == 1,
+                    "history cache rows must be contiguous in the head dimension");
+  TORCH_CHECK_TYPE(cache_k.scalar_type() == cache_v.scalar_type() && k.scalar_type() == cache_k.scalar_type() &&
+                       v.scalar_type() == cache_k.scalar_type(),
+                   "history cache, keys and values must have one dtype");
+  TORCH_CHECK_VALUE(sinks >= 0 && cache_k.size(1) > sinks, "history cache capacity must exceed its sinks");
+  TORCH_CHECK_VALUE(cache_k.size(3) >= 1 && cache_k.size(3) <= 128, "attention head dimension must be 1 to 128");
+  TORCH_CHECK_VALUE(cache_k.size(2) >= 1, "history cache needs a head");
+  same_device(cache_v, cache_k, "history cache");
+  same_device(k, cache_k, "keys");
+  same_device(v, cache_k, "values");
+  mdl_attention_step a{};
+  a.dtype = dtype_code(cache_k.scalar_type());
+  a.cache_k = cache_k.data_ptr();
+  a.cache_v = cache_v.data_ptr();
+  a.batch = cache_k.size(0);
+  a.capacity = cache_k.size(1);
+  a.kv_heads = a.q_heads = (int32_t)cache_k.size(2);
+  a.head_dim = (int32_t)cache_k.size(3);
+  a.ck_batch = cache_k.stride(0); a.ck_slot = cache_k.stride(1); a.ck_head = cache_k.stride(2);
+  a.cv_batch = cache_v.stride(0); a.cv_slot = cache_v.stride(1); a.cv_head = cache_v.stride(2);
+  a.sinks = sinks;
+  return a;
+}
+
+void check_positions(const Tensor& t, const Tensor& cache, const char* what) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kLong, what, " must be torch.long");
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == cache.size(0), what, " must hold one entry per row of the cache");
+  same_device(t, cache, what);
+}
+
+Tensor cache_step_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v,
+                       const Tensor& positions, const std::optional<Tensor>& bias_table,
+                       const std::optional<Tensor>& bucket_starts, int64_t distances, int64_t window, int64_t sinks,
+                       double scale) {
+  mdl_attention_step a = cache_args(k, v, cache_k, cache_v, sinks);
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(0) == a.batch &&
+                        k.size(0) == a.batch && k.size(1) == a.kv_heads && k.size(2) == a.head_dim &&
+                        q.size(2) == a.head_dim,
+                    "a step takes q [B, Hq, D], k and v [B, Hkv, D] of the cache's rows");
+  TORCH_CHECK_VALUE(q.size(1) > 0 && q.size(1) % a.kv_heads == 0,
+                    "attention query heads must be a multiple of the key heads");
+  TORCH_CHECK_TYPE(q.scalar_type() == cache_k.scalar_type(), "history cache and queries must have one dtype");
+  TORCH_CHECK_VALUE(window >= 0 && window <= a.capacity - sinks,
+                    "attention window must fit the cache beside its sinks");
+  TORCH_CHECK_VALUE(scale > 0 && scale < 1e30, "attention scale must be positive");
+  same_device(q, cache_k, "queries");
+  check_positions(positions, cache_k, "positions");
+  const Tensor qi = inner_contiguous(q), ki = inner_contiguous(k), vi = inner_contiguous(v);
+  const Tensor at = positions.contiguous();
+  Tensor table, starts;
+  a.q_heads = (int32_t)q.size(1);
+  if (bias_table.has_value()) {
+    bias_args(bias_table, bucket_starts, distances, q, q.size(1), table, starts);
+    a.bias_table = table.data_ptr();
+    a.bucket_starts = static_cast<const int32_t*>(starts.data_ptr());
+    a.table_dtype = dtype_code(table.scalar_type());
+    a.num_buckets = (int32_t)table.size(0);
+    a.distances = (int32_t)distances;
+  }
+  a.q = qi.data_ptr(); a.k = ki.data_ptr(); a.v = vi.data_ptr();
+  a.q_batch = qi.stride(0); a.q_head = qi.stride(1);
+  a.k_batch = ki.stride(0); a.k_head = ki.stride(1);
+  a.v_batch = vi.stride(0); a.v_head = vi.stride(1);
+  a.positions = static_cast<const int64_t*>(at.data_ptr());
+  a.window = window;
+  a.scale = (float)scale;
+  c10::DeviceGuard guard(q.device());
+  Tensor out = at::empty(q.sizes(), options_of(q, q.scalar_type()));
+  if (a.batch == 0) return out;
+  const size_t bytes = mdl_attention_step_workspace_bytes(&a);
+  Tensor ws;
+  if (bytes) ws = workspace(bytes, q.device());
+  check(mdl_attention_step_forward(&a, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q.device())),
+        "mdl_attention_step_forward");
+  return out;
+}
+
+void cache_write_cuda(const Tensor& k, const Tensor& v, const Tensor& cache_k, const Tensor& cache_v,
+                      const Tensor& lengths, int64_t sinks, bool right_aligned) {
+  mdl_attention_step a = cache_args(k, v, cache_k, cache_v, sinks);
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && k.size(0) == a.batch && k.size(2) == a.kv_heads &&
+                        k.size(3) == a.head_dim,
+                    "a prompt's k and v must be [B, L, Hkv, D] of the cache's rows");
+  check_positions(lengths, cache_k, "lengths");
+  const Tensor ki = inner_contiguous(k), vi = inner_contiguous(v), ln = lengths.contiguous();
+  a.k = ki.data_ptr(); a.v = vi.data_ptr();
+  a.k_batch = ki.stride(0); a.k_head = ki.stride(2);
+  a.v_batch = vi.stride(0); a.v_head = vi.stride(2);
+  if (k.numel() == 0) return;
+  c10::DeviceGuard guard(k.device());
+  check(mdl_attention_cache_write(&a, k.size(1), ki.stride(1), vi.stride(1), static_cast<const int64_t*>(ln.data_ptr()),
+                                  right_aligned ? 1 : 0, stream_of(k.device())),
+        "mdl_attention_cache_write");
+}
+
 }  // namespace
 }  // namespace mdl_torch
 
@@ -245,12 +349,18 @@ TORCH_LIBRARY_FRAGMENT(mdl_hip, m) {
   m.def("history_attention_backward(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor? bias_table, "
         "Tensor? bucket_starts, int distances, int window, int sinks, float scale, Tensor out, Tensor stats, "
         "Tensor prepared, bool need_table) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("history_cache_step(Tensor q, Tensor k, Tensor v, Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor positions, "
+        "Tensor? bias_table, Tensor? bucket_starts, int distances, int window, int sinks, float scale) -> Tensor");
+  m.def("history_cache_write_(Tensor k, Tensor v, Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor lengths, int sinks, "
+        "bool right_aligned) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(mdl_hip, CUDA, m) {
   using namespace mdl_torch;
   m.impl("history_attention_forward", &attention_forward_cuda);
   m.impl("history_attention_backward", &attention_backward_cuda);
+  m.impl("history_cache_step", &cache_step_cuda);
+  m.impl("history_cache_write_", &cache_write_cuda);
 }
 
 TORCH_LIBRARY_IMPL(mdl_hip, CompositeExplicitAutograd, m) {

@@ -6,11 +6,13 @@ rows and ``[B, T]`` mask, projected to heads, attend to each other.
 * :func:`history_attention` -- causal attention with a sliding window, a few
   first tokens that stay visible, heads that share keys, the lookup's mask and
   a learned relative position bias; differentiable.
+* :class:`HistoryCache` -- the keys and values of histories that grow: prompts
+  written at once, then one new token a row, which attends to what it sees.
 * :class:`RelativeBuckets` -- which distances share a learned bias.
 
 The operators are ``mdl_hip::history_attention`` (differentiable) over
-``history_attention_forward`` and ``history_attention_backward``: ROCm kernels
-in ``libmdl_torch.so`` over the C ABI, CPU kernels (PyTorch operations, for
+``history_attention_forward`` and ``history_attention_backward``,
+``history_cache_step`` and ``history_cache_write_``: ROCm kernels in ``libmdl_torch.so`` over the C ABI, CPU kernels (PyTorch operations, for
 parameters on the CPU) and fake kernels registered here.
 
 The mask marks a row's real columns.  A masked column is neither read as a key
@@ -260,6 +262,106 @@ def _attention_backward_fake(grad_out, q, k, v, mask, bias_table, bucket_starts,
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), table
 
 
+def _cache_rows_cpu(positions, capacity, sinks):
+    """(position held by each slot once position n is stored, negative: none;
+    the new token's slot) of every row."""
+
+    ring = capacity - sinks
+    slot = torch.arange(capacity)
+    n = positions[:, None]
+    held = torch.where(slot < sinks, slot, n - torch.remainder(n - slot, ring))
+    held = torch.where((slot >= sinks) & (held < sinks), -1, held)
+    at = torch.where(positions < sinks, positions, sinks + torch.remainder(positions - sinks, ring))
+    return torch.where(held > n, -1, held), at
+
+
+def _check_cache(k, v, cache_k, cache_v, sinks) -> None:
+    if cache_k.ndim != 4 or cache_k.shape != cache_v.shape:
+        raise ValueError("history cache keys and values must be [B, capacity, Hkv, D]")
+    if not cache_k.dtype == cache_v.dtype == k.dtype == v.dtype:
+        raise TypeError("history cache, keys and values must have one dtype")
+    if cache_k.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"unsupported attention dtype {cache_k.dtype}; expected float32 or bfloat16")
+    if sinks < 0 or cache_k.size(1) <= sinks:
+        raise ValueError("history cache capacity must exceed its sinks")
+    if not 1 <= cache_k.size(3) <= 128:
+        raise ValueError("attention head dimension must be 1 to 128")
+
+
+def _check_positions(t, cache, what) -> None:
+    if t.dtype != torch.long:
+        raise TypeError(f"{what} must be torch.long")
+    if t.ndim != 1 or t.size(0) != cache.size(0):
+        raise ValueError(f"{what} must hold one entry per row of the cache")
+
+
+@_cpu_kernel("history_cache_step")
+def _cache_step_cpu(q, k, v, cache_k, cache_v, positions, bias_table, bucket_starts, distances, window, sinks, scale):
+    _check_cache(k, v, cache_k, cache_v, sinks)
+    B, capacity, K, D = cache_k.shape
+    if q.ndim != 3 or k.shape != (B, K, D) or v.shape != k.shape or q.size(0) != B or q.size(2) != D:
+        raise ValueError("a step takes q [B, Hq, D], k and v [B, Hkv, D] of the cache's rows")
+    if q.size(1) == 0 or q.size(1) % K:
+        raise ValueError("attention query heads must be a multiple of the key heads")
+    if not 0 <= window <= capacity - sinks:
+        raise ValueError("attention window must fit the cache beside its sinks")
+    if not 0 < scale < 1e30:
+        raise ValueError("attention scale must be positive")
+    _check_positions(positions, cache_k, "positions")
+    if bias_table is not None:
+        _check_bias(bias_table, bucket_starts, distances, q.size(1))
+    if B == 0:
+        return torch.empty_like(q)
+    held, at = _cache_rows_cpu(positions, capacity, sinks)
+    row = (positions >= 0).nonzero().flatten()
+    cache_k[row, at[row]] = k[row]
+    cache_v[row, at[row]] = v[row]
+    distance = positions[:, None] - held
+    seen = (held >= 0) & (positions >= 0)[:, None]
+    if window:
+        seen = seen & ((distance < window) | (held < sinks))
+    kf = torch.where(seen[:, :, None, None], cache_k.float(), 0.0)
+    vf = torch.where(seen[:, :, None, None], cache_v.float(), 0.0)
+    qf = q.float().reshape(B, K, -1, D)
+    scores = torch.matmul(qf, kf.permute(0, 2, 3, 1)) * scale
+    if bias_table is not None:
+        bucket = torch.bucketize(distance.clamp(min=0), bucket_starts.long(), right=True)
+        scores = scores + bias_table.float()[bucket].reshape(B, capacity, K, -1).permute(0, 2, 3, 1)
+    scores = scores.masked_fill(~seen[:, None, None], -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    e = torch.exp(scores - torch.where(top == -math.inf, 0.0, top))
+    total = e.sum(-1, keepdim=True)
+    out = torch.matmul(e / torch.where(total == 0, 1.0, total), vf.permute(0, 2, 1, 3))
+    return out.reshape(q.shape).to(q.dtype)
+
+
+@_fake_kernel("history_cache_step")
+def _cache_step_fake(q, k, v, cache_k, cache_v, positions, bias_table, bucket_starts, distances, window, sinks, scale):
+    return q.new_empty(q.shape)
+
+
+@_cpu_kernel("history_cache_write_")
+def _cache_write_cpu(k, v, cache_k, cache_v, lengths, sinks, right_aligned):
+    _check_cache(k, v, cache_k, cache_v, sinks)
+    B, capacity, K, D = cache_k.shape
+    if k.ndim != 4 or k.shape != v.shape or k.size(0) != B or k.shape[2:] != (K, D):
+        raise ValueError("a prompt's k and v must be [B, L, Hkv, D] of the cache's rows")
+    _check_positions(lengths, cache_k, "lengths")
+    ring, L = capacity - sinks, k.size(1)
+    for b in range(B):
+        n = min(int(lengths[b]), L)
+        p = torch.arange(max(n, 0))
+        p = p[(p < sinks) | (p >= n - ring)]
+        slots = torch.where(p < sinks, p, sinks + (p - sinks) % ring)
+        rows = p + (L - n if right_aligned else 0)
+        cache_k[b, slots], cache_v[b, slots] = k[b, rows], v[b, rows]
+
+
+@_fake_kernel("history_cache_write_")
+def _cache_write_fake(k, v, cache_k, cache_v, lengths, sinks, right_aligned):
+    return None
+
+
 # ------------------------------------------------------------- attention --
 
 
@@ -317,3 +419,65 @@ def history_attention(
         scale = q.size(-1) ** -0.5 if q.ndim else 1.0
     return torch.ops.mdl_hip.history_attention(q, k, v, mask, bias_table, starts, distances, _window_argument(window),
                                                int(sinks), float(scale))
+
+
+class HistoryCache:
+    """Keys and values of histories that grow, one row per user.
+
+    ``k`` and ``v`` are ``[B, capacity, Hkv, D]``.  Position ``p`` of a row's
+    history lies in slot ``p`` while the capacity lasts; from then on new
+    positions replace the oldest ones, the first ``sinks`` excepted.  With
+    ``capacity == sinks + window`` a row keeps just what its next token sees,
+    however long its history.
+
+    Inference only: nothing here is differentiable.
+    """
+
+    def __init__(self, k: Tensor, v: Tensor, *, window: Optional[int] = None, sinks: int = 0) -> None:
+        _check_cache(k, v, k, v, sinks)
+        self._window = _window_argument(window)
+        if self._window > k.size(1) - sinks:
+            raise ValueError("attention window must fit the cache beside its sinks")
+        self.k = k
+        self.v = v
+        self.sinks = int(sinks)
+
+    @classmethod
+    def empty(cls, batch: int, capacity: int, kv_heads: int, head_dim: int, *, window: Optional[int] = None,
+              sinks: int = 0, dtype: torch.dtype = torch.float32, device=None) -> "HistoryCache":
+        shape = (batch, capacity, kv_heads, head_dim)
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                   window=window, sinks=sinks)
+
+    @property
+    def window(self) -> Optional[int]:
+        return self._window or None
+
+    @property
+    def capacity(self) -> int:
+        return self.k.size(1)
+
+    @torch.no_grad()
+    def write(self, k: Tensor, v: Tensor, lengths: Tensor, *, right_aligned: bool = False) -> None:
+        """Store prompts: ``k, v [B, L, Hkv, D]`` hold positions ``0 ..
+        lengths[b] - 1`` of each row in their first rows, or in their last
+        ones (``sequence_embedding_lookup``'s window) with ``right_aligned``."""
+
+        torch.ops.mdl_hip.history_cache_write_(k, v, self.k, self.v, lengths, self.sinks, right_aligned)
+
+    @torch.no_grad()
+    def step(self, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, *, bias_table: Optional[Tensor] = None,
+             buckets: Optional[RelativeBuckets] = None, scale: Optional[float] = None) -> Tensor:
+        """Store one new token a row and attend from it.
+
+        ``k, v [B, Hkv, D]`` are stored as position ``positions[b]``; the answer
+        to ``q [B, Hq, D]`` runs over the positions up to it that lie within
+        the window or among the sinks, as :func:`history_attention` would give
+        it.  A negative position stores nothing and is answered with zeros.
+        """
+
+        starts, distances = _bias_arguments(bias_table, buckets)
+        if scale is None:
+            scale = q.size(-1) ** -0.5
+        return torch.ops.mdl_hip.history_cache_step(q, k, v, self.k, self.v, positions, bias_table, starts, distances,
+                                                    self._window, self.sinks, float(scale))
