@@ -765,6 +765,69 @@ int mdl_attention_step_forward(const mdl_attention_step* step, void* out, void* 
 int mdl_attention_cache_write(const mdl_attention_step* step, int64_t len, int64_t k_row, int64_t v_row,
                               const int64_t* lengths, int32_t right_aligned, void* stream);
 
+/* ------------------------------------------------- relative position bias --- */
+
+/*
+ * out[h, i, j] = table[bucket(i + k_len - q_len - j), h], [heads, q_len,
+ * k_len] contiguous, in the table's dtype; table [num_buckets, heads]
+ * contiguous, q_len <= k_len.  bucket(d) = number of bucket_starts (device,
+ * ascending) at or below max(d, 0); with bidirectional the starts are those
+ * of num_buckets / 2 buckets, and a negative d takes the bucket of -d in the
+ * second half.  The gradient sums grad [heads, q_len, k_len] (contiguous,
+ * dtype) over each bucket's places, in fp32 and a fixed order.
+ */
+int mdl_relative_bias(const void* table, const int32_t* bucket_starts, int32_t num_buckets, int32_t bidirectional,
+                      int32_t heads, int64_t q_len, int64_t k_len, int32_t dtype, void* out, void* stream);
+size_t mdl_relative_bias_grad_workspace_bytes(int32_t num_buckets, int32_t heads, int64_t q_len, int64_t k_len,
+                                              int32_t dtype);
+int mdl_relative_bias_grad(const void* grad, const int32_t* bucket_starts, int32_t num_buckets, int32_t bidirectional,
+                           int32_t heads, int64_t q_len, int64_t k_len, int32_t dtype, void* grad_table,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------- norms around a block --- */
+
+/*
+ * r = block_out / rms(block_out) * post_weight
+ * y = x + sigmoid(gate) * residual_scale * r
+ * h = y / rms(y) * next_weight,      rms(v) = sqrt(mean(v^2) + eps)
+ * over rows of dim elements (x, block_out, gate, y, h: [rows, dim]
+ * contiguous, dtype; weights [dim], weight_dtype).  gate, residual_scale and
+ * the weights may be NULL (1); block_out NULL: y = x, not written, and h is
+ * its norm.  rstd [2, rows] fp32: 1 / rms of block_out and of y, written by
+ * the forward and read by the backward.
+ */
+typedef struct mdl_block_norm {
+  const void* x;
+  const void* block_out;
+  const void* gate;
+  const void* residual_scale;
+  const void* post_weight;
+  const void* next_weight;
+  float* rstd;
+  int64_t rows;
+  int32_t dim, dtype, weight_dtype;
+  float eps;
+} mdl_block_norm;
+
+int mdl_block_norm_forward(const mdl_block_norm* call, void* y, void* h, void* stream);
+
+/* grad_y or grad_h NULL: zeros.  Weight gradients (NULL: not wanted) in
+ * weight_dtype, summed in fp32 in a fixed order. */
+typedef struct mdl_block_norm_grads {
+  const void* grad_y;
+  const void* grad_h;
+  void* grad_x;
+  void* grad_block_out;
+  void* grad_gate;
+  void* grad_residual_scale;
+  void* grad_post_weight;
+  void* grad_next_weight;
+} mdl_block_norm_grads;
+
+size_t mdl_block_norm_backward_workspace_bytes(const mdl_block_norm* call);
+int mdl_block_norm_backward(const mdl_block_norm* call, const mdl_block_norm_grads* grads, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -123,6 +123,16 @@ ATTENTION_STEP_DTYPE = np.dtype(
         "q_heads", "kv_heads", "head_dim", "dtype", "table_dtype", "num_buckets", "distances")]
     + [("scale", "<f4")]
 )
+BLOCK_NORM_DTYPE = np.dtype(
+    [(name, "<u8") for name in (
+        "x", "block_out", "gate", "residual_scale", "post_weight", "next_weight", "rstd")]
+    + [("rows", "<i8"), ("dim", "<i4"), ("dtype", "<i4"), ("weight_dtype", "<i4"), ("eps", "<f4")]
+)
+BLOCK_NORM_GRADS_DTYPE = np.dtype(
+    [(name, "<u8") for name in (
+        "grad_y", "grad_h", "grad_x", "grad_block_out", "grad_gate", "grad_residual_scale", "grad_post_weight",
+        "grad_next_weight")]
+)
 assert ATTENTION_DTYPE.itemsize == 200
 assert ATTENTION_STEP_DTYPE.itemsize == 224
 assert ATTENTION_GRADS_DTYPE.itemsize == 80
@@ -209,6 +219,12 @@ SIGNATURES: dict[str, tuple] = {
     "mdl_attention_step_workspace_bytes": (_SZ, [_P]),
     "mdl_attention_step_forward": (_I32, [_P, _P, _P, _SZ, _P]),
     "mdl_attention_cache_write": (_I32, [_P, _I64, _I64, _I64, _P, _I32, _P]),
+    "mdl_relative_bias": (_I32, [_P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _P, _P]),
+    "mdl_relative_bias_grad_workspace_bytes": (_SZ, [_I32, _I32, _I64, _I64, _I32]),
+    "mdl_relative_bias_grad": (_I32, [_P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _P, _P, _SZ, _P]),
+    "mdl_block_norm_forward": (_I32, [_P, _P, _P, _P]),
+    "mdl_block_norm_backward_workspace_bytes": (_SZ, [_P]),
+    "mdl_block_norm_backward": (_I32, [_P, _P, _P, _SZ, _P]),
     "mdl_rowwise_adagrad": (
         _I32,
         [_P, _I32, _I64, _I32, _I64, _P, _P, _I64, _P, _I32, _I64, _F, _F, _P, _P],

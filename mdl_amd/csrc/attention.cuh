@@ -127,20 +127,10 @@ __device__ __forceinline__ int result_row(int i) { return 8 * (i >> 2) + 4 * (la
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The maximum, and the sum, of v over this lane and the lane 32 away.
+// The maximum of v over this lane and the lane 32 away.
 __device__ __forceinline__ float max_halves(float v) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float sum_halves(float v) {
-  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-
-// *p += v in LDS, without a result.
-__device__ __forceinline__ void lds_add(float* p, float v) {
-  typedef __attribute__((address_space(3))) float* lds_float;
-  __builtin_amdgcn_ds_faddf((lds_float)p, v, 0, 0, false);
 }
 
 // Bits [0, n) of a 32-bit word, n any.

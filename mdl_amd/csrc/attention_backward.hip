@@ -206,29 +206,6 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
   }
 }
 
-// grad_table[bucket, head]: the blocks' parts in order.  A block sums 8
-// buckets of one head, 32 threads each.
-template <typename TB>
-__global__ __launch_bounds__(256) void bias_partial_sum_kernel(const float* partial, int64_t parts, int buckets,
-                                                               int heads, TB* grad) {
-  __shared__ float smem[256];
-  const int head = blockIdx.y, k = blockIdx.x * 8 + (threadIdx.x & 7), part = threadIdx.x >> 3;
-  float s = 0.f;
-  if (k < buckets) {
-    const float* p = partial + (int64_t)head * parts * buckets + k;
-#pragma unroll 4
-    for (int64_t i = part; i < parts; i += 32) s += p[i * buckets];
-  }
-  smem[threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.x < 8 && k < buckets) {
-    double t = 0.;
-    for (int i = 0; i < 32; ++i) t += (double)smem[8 * i + threadIdx.x];
-    if constexpr (sizeof(TB) == 2) grad[(int64_t)k * heads + head] = f32_to_bf16((float)t);
-    else grad[(int64_t)k * heads + head] = (float)t;
-  }
-}
-
 // ---------------------------------------------------------- keys: dk and dv --
 
 // kFar: the pairs of the first tokens and the queries a window or more past
@@ -550,14 +527,8 @@ int mdl_attention_backward(const mdl_attention* a, const void* prepared, const m
       }))
     return rc;
   if (grads->grad_table) {
-    const dim3 grid((unsigned)((a->num_buckets + 7) / 8), (unsigned)a->q_heads);
-    if (a->table_dtype == MDL_F32)
-      hipLaunchKernelGGL(bias_partial_sum_kernel<float>, grid, dim3(256), 0, s, g.bias_partial, lay.bias_parts,
-                         a->num_buckets, a->q_heads, static_cast<float*>(grads->grad_table));
-    else
-      hipLaunchKernelGGL(bias_partial_sum_kernel<bf16_t>, grid, dim3(256), 0, s, g.bias_partial, lay.bias_parts,
-                         a->num_buckets, a->q_heads, static_cast<bf16_t*>(grads->grad_table));
-    MDL_CHECK_LAUNCH("bias_partial_sum_kernel");
+    return sum_bias_parts(g.bias_partial, lay.bias_parts, a->num_buckets, a->q_heads, a->table_dtype,
+                          grads->grad_table, s);
   }
   return MDL_OK;
 }

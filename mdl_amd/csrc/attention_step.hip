@@ -59,23 +59,6 @@ struct StepRows {
   }
 };
 
-// Sum over aligned groups of N lanes, in every lane.
-template <int N>
-__device__ __forceinline__ float group_sum(float v) {
-  auto dpp = [&](auto ctrl) {
-    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
-  };
-  if constexpr (N >= 2) v += dpp(std::integral_constant<int, 0xB1>{});   // quad: 1 0 3 2
-  if constexpr (N >= 4) v += dpp(std::integral_constant<int, 0x4E>{});   // quad: 2 3 0 1
-  if constexpr (N >= 8) v += dpp(std::integral_constant<int, 0x141>{});  // mirror of 8
-  if constexpr (N >= 16) v += dpp(std::integral_constant<int, 0x140>{}); // mirror of 16
-  if constexpr (N >= 32) {
-    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-  }
-  return v;
-}
-
 template <typename T>
 __device__ __forceinline__ float element(const typename Frags<T>::Frag& f, int i) {
   return (float)f[i];

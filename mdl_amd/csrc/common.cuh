@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <string>
+#include <type_traits>
 
 #include "../../include/mdl_hip.h"
 
@@ -34,6 +35,11 @@ struct ClipTail {
   float* total_norm = nullptr;
   float* coef = nullptr;
 };
+
+// The bias table's gradient [buckets, heads] from parts [heads, parts,
+// buckets], added in order.
+int sum_bias_parts(const float* partial, int64_t parts, int32_t buckets, int32_t heads, int32_t dtype, void* grad,
+                   hipStream_t s);
 
 static inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
@@ -436,6 +442,35 @@ __device__ __forceinline__ uint32_t shfl_u(uint32_t v, int src) {
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// *p += v in LDS, without a result.
+__device__ __forceinline__ void lds_add(float* p, float v) {
+  typedef __attribute__((address_space(3))) float* lds_float;
+  __builtin_amdgcn_ds_faddf((lds_float)p, v, 0, 0, false);
+}
+
+// The sum of v over this lane and the lane 32 away.
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// Sum over aligned groups of N lanes, in every lane.
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+  auto dpp = [&](auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if constexpr (N >= 2) v += dpp(std::integral_constant<int, 0xB1>{});   // quad: 1 0 3 2
+  if constexpr (N >= 4) v += dpp(std::integral_constant<int, 0x4E>{});   // quad: 2 3 0 1
+  if constexpr (N >= 8) v += dpp(std::integral_constant<int, 0x141>{});  // mirror of 8
+  if constexpr (N >= 16) v += dpp(std::integral_constant<int, 0x140>{}); // mirror of 16
+  if constexpr (N >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
 }
 
 // Lanes per row: next power of two >= ceil(dim / C), capped at one wave.

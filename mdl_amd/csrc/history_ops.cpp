@@ -1,8 +1,10 @@
 // Operators over long histories (namespace mdl_hip), in C++: the window
-// attention with its gradient.  Each operator's ROCm kernel calls the C ABI of
-// libmdl_hip.so on the current HIP stream; CPU and fake kernels are registered
-// by mdl_amd/history.py on these schemas.  The gradient is an autograd node
-// made here, so that a training step's Python is one call.
+// attention, its single-token form over a cache, the relative position bias
+// and the norms around a block.  Each operator's ROCm kernel calls the C ABI
+// of libmdl_hip.so on the current HIP stream; CPU and fake kernels are
+// registered by mdl_amd/history.py and mdl_amd/block_norm.py on these schemas.
+// Gradients are autograd nodes made here, so that a training step's Python is
+// one call.
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -183,13 +185,6 @@ std::tuple<Tensor, Tensor, Tensor> call_attention_forward(
   return op.call(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale, need_backward);
 }
 
-Tensor history_attention_plain(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
-                               const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts,
-                               int64_t distances, int64_t window, int64_t sinks, double scale) {
-  return std::get<0>(call_attention_forward(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale,
-                                            false));
-}
-
 std::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
@@ -206,6 +201,7 @@ struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["need_table"] = bias_table.has_value() && bias_table->requires_grad();
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -213,13 +209,14 @@ struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("mdl_hip::history_attention_backward", "")
                                .typed<decltype(attention_backward_cuda)>();
+    const bool need_table = ctx->saved_data["need_table"].toBool();
     auto [dq, dk, dv, dtable] =
         op.call(grads[0], s[0], s[1], s[2], optional_of(s[3]), optional_of(s[4]), optional_of(s[5]),
                 ctx->saved_data["distances"].toInt(), ctx->saved_data["window"].toInt(),
                 ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble(), s[6], s[7], s[8],
-                s[4].defined() && ctx->needs_input_grad(4));
+                need_table);
     const Tensor none;
-    return {dq, dk, dv, none, s[4].defined() && ctx->needs_input_grad(4) ? dtable : none, none, none, none, none, none};
+    return {dq, dk, dv, none, need_table ? dtable : none, none, none, none, none, none};
   }
 };
 
@@ -230,7 +227,8 @@ Tensor history_attention_autograd(const Tensor& q, const Tensor& k, const Tensor
                                                    (bias_table.has_value() && bias_table->requires_grad()));
   if (need) return HistoryAttention::apply(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
   at::AutoDispatchBelowADInplaceOrView below;
-  return history_attention_plain(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
+  return std::get<0>(
+      call_attention_forward(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale, false));
 }
 
 // ------------------------------------------------------ single new tokens --
@@ -337,12 +335,264 @@ void cache_write_cuda(const Tensor& k, const Tensor& v, const Tensor& cache_k, c
         "mdl_attention_cache_write");
 }
 
+// --------------------------------------------------- relative position bias --
+
+void check_bias(const Tensor& table, const Tensor& starts, bool bidirectional, int64_t q_len, int64_t k_len) {
+  require_device(table, "bias table");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1, "bias table must be [buckets, heads]");
+  dtype_code(table.scalar_type());
+  same_device(starts, table, "bucket_starts");
+  const int64_t side = bidirectional ? table.size(0) / 2 : table.size(0);
+  TORCH_CHECK_VALUE(starts.scalar_type() == at::kInt && starts.dim() == 1 && starts.is_contiguous() &&
+                        starts.size(0) == side - 1 && side * (bidirectional ? 2 : 1) == table.size(0),
+                    "bucket_starts must be contiguous int32 with one entry fewer than a direction has buckets");
+  TORCH_CHECK_VALUE(q_len >= 0 && q_len <= k_len, "a relative bias has 0 <= q_len <= k_len");
+}
+
+Tensor relative_bias_cuda(const Tensor& table, const Tensor& starts, bool bidirectional, int64_t q_len, int64_t k_len) {
+  check_bias(table, starts, bidirectional, q_len, k_len);
+  c10::DeviceGuard guard(table.device());
+  const Tensor t = table.contiguous();
+  Tensor out = at::empty({t.size(1), q_len, k_len}, options_of(t, t.scalar_type()));
+  check(mdl_relative_bias(t.data_ptr(), static_cast<const int32_t*>(starts.data_ptr()), (int32_t)t.size(0),
+                          bidirectional, (int32_t)t.size(1), q_len, k_len, dtype_code(t.scalar_type()), out.data_ptr(),
+                          stream_of(t.device())),
+        "mdl_relative_bias");
+  return out;
+}
+
+Tensor relative_bias_grad_cuda(const Tensor& grad, const Tensor& starts, int64_t num_buckets, bool bidirectional) {
+  require_device(grad, "bias gradient");
+  TORCH_CHECK_VALUE(grad.dim() == 3 && grad.size(0) >= 1, "bias gradient must be [heads, q_len, k_len]");
+  same_device(starts, grad, "bucket_starts");
+  const int64_t side = bidirectional ? num_buckets / 2 : num_buckets;
+  TORCH_CHECK_VALUE(starts.scalar_type() == at::kInt && starts.is_contiguous() && starts.numel() == side - 1,
+                    "bucket_starts must be contiguous int32 with one entry fewer than a direction has buckets");
+  const int32_t dtype = dtype_code(grad.scalar_type());
+  c10::DeviceGuard guard(grad.device());
+  const Tensor g = grad.contiguous();
+  Tensor out = at::empty({num_buckets, g.size(0)}, options_of(g, g.scalar_type()));
+  const size_t bytes =
+      mdl_relative_bias_grad_workspace_bytes((int32_t)num_buckets, (int32_t)g.size(0), g.size(1), g.size(2), dtype);
+  Tensor ws = workspace(bytes, g.device());
+  check(mdl_relative_bias_grad(g.data_ptr(), static_cast<const int32_t*>(starts.data_ptr()), (int32_t)num_buckets,
+                               bidirectional, (int32_t)g.size(0), g.size(1), g.size(2), dtype, out.data_ptr(),
+                               ws.data_ptr(), bytes, stream_of(g.device())),
+        "mdl_relative_bias_grad");
+  return out;
+}
+
+Tensor call_relative_bias(const Tensor& table, const Tensor& starts, bool bidirectional, int64_t q_len, int64_t k_len) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("mdl_hip::relative_position_bias_forward", "")
+                             .typed<decltype(relative_bias_cuda)>();
+  return op.call(table, starts, bidirectional, q_len, k_len);
+}
+
+struct RelativeBias : public torch::autograd::Function<RelativeBias> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& starts, bool bidirectional,
+                        int64_t q_len, int64_t k_len) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({starts});
+    ctx->saved_data["buckets"] = table.size(0);
+    ctx->saved_data["bidirectional"] = bidirectional;
+    return call_relative_bias(table, starts, bidirectional, q_len, k_len);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("mdl_hip::relative_position_bias_backward", "")
+                               .typed<decltype(relative_bias_grad_cuda)>();
+    const Tensor none;
+    return {op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["buckets"].toInt(),
+                    ctx->saved_data["bidirectional"].toBool()),
+            none, none, none, none};
+  }
+};
+
+Tensor relative_bias_autograd(const Tensor& table, const Tensor& starts, bool bidirectional, int64_t q_len,
+                              int64_t k_len) {
+  if (at::GradMode::is_enabled() && table.requires_grad())
+    return RelativeBias::apply(table, starts, bidirectional, q_len, k_len);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_relative_bias(table, starts, bidirectional, q_len, k_len);
+}
+
+// ------------------------------------------------------ norms around a block --
+
+struct NormArgs {
+  Tensor x, o, gate, scale, post, next;
+  mdl_block_norm call{};
+};
+
+NormArgs norm_args(const Tensor& x, const std::optional<Tensor>& block_out, const std::optional<Tensor>& post_weight,
+                   const Tensor& next_weight, const std::optional<Tensor>& gate,
+                   const std::optional<Tensor>& residual_scale, double eps) {
+  require_device(x, "block norm input");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "block norm input needs a last dimension");
+  TORCH_CHECK_VALUE(eps >= 0, "block norm eps must not be negative");
+  TORCH_CHECK_VALUE(block_out.has_value() || (!post_weight.has_value() && !gate.has_value() && !residual_scale.has_value()),
+                    "gate, residual_scale and post_weight belong to a block's output");
+  NormArgs a;
+  const int64_t dim = x.size(-1);
+  auto rows = [&](const Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(t.sizes() == x.sizes(), what, " must have the input's shape");
+    TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), what, " must have the input's dtype");
+    same_device(t, x, what);
+    return t.contiguous();
+  };
+  auto weight = [&](const Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == dim, what, " must be [", dim, "]");
+    TORCH_CHECK_TYPE(t.scalar_type() == next_weight.scalar_type(), "block norm weights must have one dtype");
+    same_device(t, x, what);
+    return t.contiguous();
+  };
+  a.x = x.contiguous();
+  a.next = weight(next_weight, "next_weight");
+  if (block_out.has_value()) a.o = rows(*block_out, "block_out");
+  if (gate.has_value()) a.gate = rows(*gate, "gate");
+  if (residual_scale.has_value()) a.scale = weight(*residual_scale, "residual_scale");
+  if (post_weight.has_value()) a.post = weight(*post_weight, "post_weight");
+  auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  mdl_block_norm& c = a.call;
+  c.x = at(a.x); c.block_out = at(a.o); c.gate = at(a.gate);
+  c.residual_scale = at(a.scale); c.post_weight = at(a.post); c.next_weight = at(a.next);
+  c.dim = (int32_t)dim;
+  c.rows = x.numel() / dim;
+  c.dtype = dtype_code(x.scalar_type());
+  c.weight_dtype = dtype_code(next_weight.scalar_type());
+  c.eps = (float)eps;
+  TORCH_CHECK_VALUE(dim <= (c.dtype == MDL_BF16 ? 8192 : 4096),
+                    "block norm rows hold at most 8192 (bfloat16) or 4096 (float32) elements");
+  return a;
+}
+
+std::tuple<Tensor, Tensor, Tensor> block_norm_forward_cuda(
+    const Tensor& x, const std::optional<Tensor>& block_out, const std::optional<Tensor>& post_weight,
+    const Tensor& next_weight, const std::optional<Tensor>& gate, const std::optional<Tensor>& residual_scale,
+    double eps) {
+  NormArgs a = norm_args(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
+  c10::DeviceGuard guard(x.device());
+  Tensor y = a.o.defined() ? at::empty(x.sizes(), options_of(x, x.scalar_type()))
+                           : at::empty({0}, options_of(x, x.scalar_type()));
+  Tensor h = at::empty(x.sizes(), options_of(x, x.scalar_type()));
+  Tensor rstd = at::empty({2, a.call.rows}, options_of(x, at::kFloat));
+  if (a.call.rows == 0) return {y, h, rstd};
+  a.call.rstd = static_cast<float*>(rstd.data_ptr());
+  check(mdl_block_norm_forward(&a.call, a.o.defined() ? y.data_ptr() : nullptr, h.data_ptr(), stream_of(x.device())),
+        "mdl_block_norm_forward");
+  return {y, h, rstd};
+}
+
+// needs: residual_scale, post_weight, next_weight (bits 0 to 2).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> block_norm_backward_cuda(
+    const std::optional<Tensor>& grad_y, const std::optional<Tensor>& grad_h, const Tensor& x,
+    const std::optional<Tensor>& block_out, const std::optional<Tensor>& post_weight, const Tensor& next_weight,
+    const std::optional<Tensor>& gate, const std::optional<Tensor>& residual_scale, const Tensor& rstd, double eps,
+    int64_t needs) {
+  NormArgs a = norm_args(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
+  TORCH_CHECK_VALUE(rstd.numel() == 2 * a.call.rows && rstd.is_contiguous() && rstd.scalar_type() == at::kFloat,
+                    "block norm backward needs the forward's statistics");
+  a.call.rstd = static_cast<float*>(rstd.data_ptr());
+  c10::DeviceGuard guard(x.device());
+  Tensor dy, dh;
+  auto incoming = [&](const std::optional<Tensor>& t) {
+    if (!t.has_value() || !t->defined()) return Tensor();
+    TORCH_CHECK_VALUE(t->sizes() == x.sizes(), "block norm gradients must have the input's shape");
+    TORCH_CHECK_TYPE(t->scalar_type() == x.scalar_type(), "block norm gradients must have the input's dtype");
+    same_device(*t, x, "block norm gradient");
+    return t->contiguous();
+  };
+  dy = incoming(grad_y);
+  dh = incoming(grad_h);
+  auto like_x = [&](bool want) {
+    return want ? at::empty(x.sizes(), options_of(x, x.scalar_type())) : at::empty({0}, options_of(x, x.scalar_type()));
+  };
+  auto like_w = [&](bool want) {
+    return at::empty({want ? (int64_t)a.call.dim : 0}, options_of(x, next_weight.scalar_type()));
+  };
+  Tensor dx = like_x(true), d_o = like_x(a.o.defined()), dgate = like_x(a.gate.defined());
+  Tensor dscale = like_w(a.scale.defined() && (needs & 1)), dpost = like_w(a.post.defined() && (needs & 2)),
+         dnext = like_w(needs & 4);
+  auto ptr = [](const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; };
+  mdl_block_norm_grads g{};
+  g.grad_y = ptr(dy); g.grad_h = ptr(dh);
+  g.grad_x = ptr(dx); g.grad_block_out = ptr(d_o); g.grad_gate = ptr(dgate);
+  g.grad_residual_scale = ptr(dscale); g.grad_post_weight = ptr(dpost); g.grad_next_weight = ptr(dnext);
+  const size_t bytes = mdl_block_norm_backward_workspace_bytes(&a.call);
+  Tensor ws = workspace(bytes, x.device());
+  check(mdl_block_norm_backward(&a.call, &g, ws.data_ptr(), bytes, stream_of(x.device())), "mdl_block_norm_backward");
+  return {dx, d_o, dgate, dscale, dpost, dnext};
+}
+
+std::tuple<Tensor, Tensor, Tensor> call_block_norm(
+    const Tensor& x, const std::optional<Tensor>& block_out, const std::optional<Tensor>& post_weight,
+    const Tensor& next_weight, const std::optional<Tensor>& gate, const std::optional<Tensor>& residual_scale,
+    double eps) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("mdl_hip::block_norm_forward", "")
+                             .typed<decltype(block_norm_forward_cuda)>();
+  return op.call(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
+}
+
+struct BlockNorm : public torch::autograd::Function<BlockNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& block_out,
+                               const std::optional<Tensor>& post_weight, const Tensor& next_weight,
+                               const std::optional<Tensor>& gate, const std::optional<Tensor>& residual_scale,
+                               double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, h, rstd] = call_block_norm(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, block_out.value_or(Tensor()), post_weight.value_or(Tensor()), next_weight,
+                            gate.value_or(Tensor()), residual_scale.value_or(Tensor()), rstd});
+    ctx->saved_data["eps"] = eps;
+    auto wants = [](const std::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
+    ctx->saved_data["needs"] = int64_t((wants(residual_scale) ? 1 : 0) | (wants(post_weight) ? 2 : 0) |
+                                       (next_weight.requires_grad() ? 4 : 0));
+    if (!block_out.has_value()) return {h};
+    return {y, h};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor none;
+    const auto s = ctx->get_saved_variables();
+    const bool two = s[1].defined();
+    const Tensor dy = two ? grads[0] : none, dh = grads[two ? 1 : 0];
+    if (!dy.defined() && !dh.defined()) return {none, none, none, none, none, none, none};
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("mdl_hip::block_norm_backward", "")
+                               .typed<decltype(block_norm_backward_cuda)>();
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    auto [dx, d_o, dgate, dscale, dpost, dnext] =
+        op.call(optional_of(dy), optional_of(dh), s[0], optional_of(s[1]), optional_of(s[2]), s[3], optional_of(s[4]),
+                optional_of(s[5]), s[6], ctx->saved_data["eps"].toDouble(), needs);
+    return {dx, two ? d_o : none, needs & 2 ? dpost : none, needs & 4 ? dnext : none, s[4].defined() ? dgate : none,
+            needs & 1 ? dscale : none, none};
+  }
+};
+
+// (y, h); y is x itself without a block's output.
+std::tuple<Tensor, Tensor> block_norm_autograd(const Tensor& x, const std::optional<Tensor>& block_out,
+                                               const std::optional<Tensor>& post_weight, const Tensor& next_weight,
+                                               const std::optional<Tensor>& gate,
+                                               const std::optional<Tensor>& residual_scale, double eps) {
+  auto wants = [](const std::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (x.requires_grad() || next_weight.requires_grad() || wants(block_out) ||
+                                     wants(post_weight) || wants(gate) || wants(residual_scale))) {
+    auto out = BlockNorm::apply(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
+    if (!block_out.has_value()) return {x, out[0]};
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto [y, h, rstd] = call_block_norm(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
+  return {block_out.has_value() ? y : x, h};
+}
+
 }  // namespace
 }  // namespace mdl_torch
 
 TORCH_LIBRARY_FRAGMENT(mdl_hip, m) {
   m.def("history_attention(Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor? bias_table, Tensor? bucket_starts, "
-        "int distances, int window, int sinks, float scale) -> Tensor");
+        "int distances, int window, int sinks, float scale) -> Tensor",
+        &mdl_torch::history_attention_autograd);
   m.def("history_attention_forward(Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor? bias_table, "
         "Tensor? bucket_starts, int distances, int window, int sinks, float scale, bool need_backward) "
         "-> (Tensor, Tensor, Tensor)");
@@ -353,6 +603,20 @@ TORCH_LIBRARY_FRAGMENT(mdl_hip, m) {
         "Tensor? bias_table, Tensor? bucket_starts, int distances, int window, int sinks, float scale) -> Tensor");
   m.def("history_cache_write_(Tensor k, Tensor v, Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor lengths, int sinks, "
         "bool right_aligned) -> ()");
+  m.def("relative_position_bias(Tensor table, Tensor bucket_starts, bool bidirectional, int q_len, int k_len) -> Tensor",
+        &mdl_torch::relative_bias_autograd);
+  m.def("relative_position_bias_forward(Tensor table, Tensor bucket_starts, bool bidirectional, int q_len, int k_len) "
+        "-> Tensor");
+  m.def("relative_position_bias_backward(Tensor grad, Tensor bucket_starts, int num_buckets, bool bidirectional) "
+        "-> Tensor");
+  m.def("gated_residual_norm(Tensor x, Tensor? block_out, Tensor? post_weight, Tensor next_weight, Tensor? gate, "
+        "Tensor? residual_scale, float eps) -> (Tensor, Tensor)",
+        &mdl_torch::block_norm_autograd);
+  m.def("block_norm_forward(Tensor x, Tensor? block_out, Tensor? post_weight, Tensor next_weight, Tensor? gate, "
+        "Tensor? residual_scale, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("block_norm_backward(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor? block_out, Tensor? post_weight, "
+        "Tensor next_weight, Tensor? gate, Tensor? residual_scale, Tensor rstd, float eps, int needs) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mdl_hip, CUDA, m) {
@@ -361,10 +625,8 @@ TORCH_LIBRARY_IMPL(mdl_hip, CUDA, m) {
   m.impl("history_attention_backward", &attention_backward_cuda);
   m.impl("history_cache_step", &cache_step_cuda);
   m.impl("history_cache_write_", &cache_write_cuda);
+  m.impl("relative_position_bias_forward", &relative_bias_cuda);
+  m.impl("relative_position_bias_backward", &relative_bias_grad_cuda);
+  m.impl("block_norm_forward", &block_norm_forward_cuda);
+  m.impl("block_norm_backward", &block_norm_backward_cuda);
 }
-
-TORCH_LIBRARY_IMPL(mdl_hip, CompositeExplicitAutograd, m) {
-  m.impl("history_attention", &mdl_torch::history_attention_plain);
-}
-
-TORCH_LIBRARY_IMPL(mdl_hip, Autograd, m) { m.impl("history_attention", &mdl_torch::history_attention_autograd); }

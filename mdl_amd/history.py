@@ -8,11 +8,14 @@ rows and ``[B, T]`` mask, projected to heads, attend to each other.
   a learned relative position bias; differentiable.
 * :class:`HistoryCache` -- the keys and values of histories that grow: prompts
   written at once, then one new token a row, which attends to what it sees.
-* :class:`RelativeBuckets` -- which distances share a learned bias.
+* :class:`RelativeBuckets` -- which distances share a learned bias, and
+  :func:`relative_position_bias`, that bias made whole for an attention that
+  takes it as a tensor; differentiable.
 
 The operators are ``mdl_hip::history_attention`` (differentiable) over
 ``history_attention_forward`` and ``history_attention_backward``,
-``history_cache_step`` and ``history_cache_write_``: ROCm kernels in ``libmdl_torch.so`` over the C ABI, CPU kernels (PyTorch operations, for
+``history_cache_step``, ``history_cache_write_`` and
+``relative_position_bias`` (over its ``_forward`` and ``_backward``): ROCm kernels in ``libmdl_torch.so`` over the C ABI, CPU kernels (PyTorch operations, for
 parameters on the CPU) and fake kernels registered here.
 
 The mask marks a row's real columns.  A masked column is neither read as a key
@@ -362,6 +365,52 @@ def _cache_write_fake(k, v, cache_k, cache_v, lengths, sinks, right_aligned):
     return None
 
 
+def _bias_buckets_cpu(bucket_starts, bidirectional, side, q_len, k_len):
+    column = torch.arange(k_len)
+    distance = column[k_len - q_len:, None] - column
+    near = distance.abs() if bidirectional else distance.clamp(min=0)
+    bucket = torch.bucketize(near, bucket_starts.long(), right=True)
+    return torch.where(distance < 0, bucket + side, bucket) if bidirectional else bucket
+
+
+def _check_relative_bias(table, bucket_starts, bidirectional, q_len, k_len) -> None:
+    if table.ndim != 2 or table.size(0) < 1 or table.size(1) < 1:
+        raise ValueError("bias table must be [buckets, heads]")
+    if table.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"unsupported bias dtype {table.dtype}; expected float32 or bfloat16")
+    side = table.size(0) // 2 if bidirectional else table.size(0)
+    if bucket_starts.numel() != side - 1 or side * (2 if bidirectional else 1) != table.size(0):
+        raise ValueError("bucket_starts must have one entry fewer than a direction has buckets")
+    if not 0 <= q_len <= k_len:
+        raise ValueError("a relative bias has 0 <= q_len <= k_len")
+
+
+@_cpu_kernel("relative_position_bias_forward")
+def _relative_bias_cpu(table, bucket_starts, bidirectional, q_len, k_len):
+    _check_relative_bias(table, bucket_starts, bidirectional, q_len, k_len)
+    bucket = _bias_buckets_cpu(bucket_starts, bidirectional, table.size(0) // 2, q_len, k_len)
+    return table.t()[:, bucket].contiguous()
+
+
+@_fake_kernel("relative_position_bias_forward")
+def _relative_bias_fake(table, bucket_starts, bidirectional, q_len, k_len):
+    return table.new_empty((table.size(1), q_len, k_len))
+
+
+@_cpu_kernel("relative_position_bias_backward")
+def _relative_bias_backward_cpu(grad, bucket_starts, num_buckets, bidirectional):
+    heads, q_len, k_len = grad.shape
+    bucket = _bias_buckets_cpu(bucket_starts, bidirectional, num_buckets // 2, q_len, k_len)
+    sums = torch.zeros(num_buckets, heads)
+    sums.index_add_(0, bucket.reshape(-1), grad.float().reshape(heads, -1).t())
+    return sums.to(grad.dtype)
+
+
+@_fake_kernel("relative_position_bias_backward")
+def _relative_bias_backward_fake(grad, bucket_starts, num_buckets, bidirectional):
+    return grad.new_empty((num_buckets, grad.size(0)))
+
+
 # ------------------------------------------------------------- attention --
 
 
@@ -419,6 +468,17 @@ def history_attention(
         scale = q.size(-1) ** -0.5 if q.ndim else 1.0
     return torch.ops.mdl_hip.history_attention(q, k, v, mask, bias_table, starts, distances, _window_argument(window),
                                                int(sinks), float(scale))
+
+
+def relative_position_bias(table: Tensor, q_len: int, k_len: int, buckets: RelativeBuckets) -> Tensor:
+    """``[heads, q_len, k_len]`` bias of ``table [buckets, heads]``: the value of
+    ``buckets.of(i + k_len - q_len - j)`` at ``[h, i, j]``, in the table's
+    dtype; its gradient sums over each bucket's places."""
+
+    if table.ndim != 2 or table.size(0) != buckets.num_buckets:
+        raise ValueError(f"bias table must have one row for each of the {buckets.num_buckets} buckets")
+    return torch.ops.mdl_hip.relative_position_bias(table, buckets.starts_on(table.device), buckets.bidirectional,
+                                                    int(q_len), int(k_len))
 
 
 class HistoryCache:
