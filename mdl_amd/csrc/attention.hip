@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
   const float* bias = a.bias ? a.bias + (int64_t)head * a.distances : nullptr;
 
   const int off = a.k_len - a.q_len;
-  const int wave = threadIdx.x / kWave, l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
   const int r0 = qb * kAttnRows;
   const int r_end = r0 + kAttnRows < a.q_len ? r0 + kAttnRows : a.q_len;
   const int row = r0 + 32 * wave + l32, c = row + off;
@@ -132,6 +132,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
   const float lazy = kLazyRaise / a.c2;
 
   const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
+  const f32x16 far_bias = (f32x16)(bias ? bias[a.distances - 1] : 0.f);
   Stage ks, vs;
   float bias_next = 0.f;
   auto fetch = [&](int t, uint64_t bits) {
@@ -163,21 +164,24 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
     const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
     if (seen) {
       f32x16 x[kSubs];
+      auto products = [&](int s, f32x16 from) {
+        x[s] = F::mma(load_frag(lk + nat + 32 * s * LD), q[0], from);
+#pragma unroll
+        for (int d = 1; d < kSteps; ++d) x[s] = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x[s]);
+      };
       // distances of the wave and the tile all in the last bucket, or none told apart
-      const bool flat = !bias || wc_lo - j1 >= a.distances - 1;
-      const float flat_bias = bias ? lb[kAttnRows - 32 - 32 * wave] : 0.f;
+      if (!bias || wc_lo - j1 >= a.distances - 1) {
 #pragma unroll
-      for (int s = 0; s < kSubs; ++s) {
-        if (flat) {
-          x[s] = (f32x16)(flat_bias);
-        } else {
+        for (int s = 0; s < kSubs; ++s) products(s, far_bias);
+      } else {
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s) {
           const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
+          f32x16 near;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[s][i] = from[8 * (i >> 2) + (i & 3)];
+          for (int i = 0; i < 16; ++i) near[i] = from[8 * (i >> 2) + (i & 3)];
+          products(s, near);
         }
-#pragma unroll
-        for (int d = 0; d < kSteps; ++d)
-          x[s] = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x[s]);
       }
       const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
                          wc_lo + 31 - j0 < a.window;
@@ -229,8 +233,9 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
 
   l = sum_halves(l);
   if (row < a.q_len) {
-    store_result_row<T, DP>(out + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim, acc,
-                            l > 0.f ? 1.f / l : 0.f, a.dim);
+    const int64_t at = (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    store_result_row<T, DP>(out + at, acc, inv, a.dim);
     if (stats && half == 0) {
       // log2 of the sum at the unrounded c2 m; +inf makes every weight of an empty row 0
       const float ll = l > 0.f ? log2f(l) - __builtin_fmaf(m, a.c2, mneg) : INFINITY;

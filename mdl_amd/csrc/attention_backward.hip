@@ -1,14 +1,22 @@
 // Gradients of the history attention.
 //
 // With p the forward's weights (made again from q, k and the saved row
-// statistics), dP = dO . v and delta = sum p dP = dO . out of a row:
+// statistics), dP = dO . v and delta = sum p dP of a row:
 //   dS = p (dP - delta),  dq = scale sum_k dS k,  dk = scale sum_q dS q,
 //   dv = sum_q p dO,      dbias[bucket] = sum of dS over the bucket's places.
 // Two kernels, so that every sum has one owner and a fixed order: one walks
-// the keys of 128 queries (dq, delta and the bias), one the queries of 128
-// keys (dk and dv, over all heads that share the keys).  Making the weights
-// twice costs seven products instead of five; adding dq across blocks
-// instead would need atomics, whose order changes results.
+// the keys of 128 queries (dq and delta), then one the queries of 128 keys (dk
+// and dv over all heads that share the keys, and the bias).  Making the
+// weights twice costs two products more than making them once; adding dq
+// across blocks instead would need atomics, whose order changes results.
+//
+// delta.  dO . out is delta up to the rounding of out, and of the weights
+// that out was made from, to bfloat16: an error of the size of dS's own
+// rounding, and larger in rows whose dS cancel.  The first kernel works with it
+// all the same, adds the row's dS in fp32 to what it is short of (their sum
+// is 0 with the true delta), and takes the share of k that belongs to the
+// difference (a fourth product, sum p k) off dq at the end; the second kernel
+// reads the corrected delta.
 #include "attention.cuh"
 
 namespace mdl {
@@ -22,15 +30,17 @@ struct GradCall {
   float* delta;         // [B, Hq, Lq]
   const int32_t* starts;
   int32_t buckets;
-  float* bias_partial;  // [Hq, B * blocks_q, buckets]; NULL: no bias gradient
+  float* bias_partial;  // [Hq, bias_parts, buckets]; NULL: no bias gradient
+  int64_t bias_parts, bias_far;  // parts of a head; the first one of the far blocks
   float* far_partial;   // [B, Hkv, far_chunks, sinks, 2, dim]; NULL: no far part
   int32_t far_chunks;
 };
 
 constexpr int kSpare = 96;      // distances of one tile and wave past either end of the bias
 constexpr int kFarRows = 512;   // query rows of a block of the first tokens' far part
+constexpr int kSkew = 64;       // diagonals of a 32x32 product tile, padded
 
-// ------------------------------------------------- queries: dq, delta, bias --
+// ------------------------------------------------------ queries: dq, delta --
 
 template <typename T, int DP, bool kVec>
 __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall a, GradCall g) {
@@ -41,10 +51,6 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
   extern __shared__ __align__(16) char smem[];
   T* lds = reinterpret_cast<T*>(smem);
   float* lds_bias = reinterpret_cast<float*>(lds + 4 * TK * LD);
-  // bias gradient by distance: one array per wave and half wave, so that the
-  // lanes of one addition never meet and every array is added to in order
-  float* lds_sum = lds_bias + 2 * kBias;
-  const int n_sum = g.bias_partial ? a.distances + 2 * kSpare : 0;
 
   const int blocks_q = (a.q_len + kAttnRows - 1) / kAttnRows;
   int64_t id = xcd_block(blockIdx.x, gridDim.x);
@@ -57,7 +63,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
   const float* bias = a.bias ? a.bias + (int64_t)head * a.distances : nullptr;
 
   const int off = a.k_len - a.q_len;
-  const int wave = threadIdx.x / kWave, l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
   const int r0 = qb * kAttnRows;
   const int r_end = r0 + kAttnRows < a.q_len ? r0 + kAttnRows : a.q_len;
   const int row = r0 + 32 * wave + l32, c = row + off;
@@ -73,7 +79,6 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
       static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head + (int64_t)row * g.g_row, live, a.dim, go);
   float m = 0.f, ll = INFINITY, delta = 0.f;
   {
-    const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + row;
     typename F::Frag o[kSteps];
     load_own_row<T, DP, kVec>(static_cast<const T*>(g.out) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim,
                               live, a.dim, o);
@@ -83,18 +88,16 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
       for (int i = 0; i < F::kElems; ++i) delta += (float)o[s][i] * (float)go[s][i];
     delta = sum_halves(delta);
     if (row < a.q_len) {
-      const float2 st = g.stats[at];
+      const float2 st = g.stats[((int64_t)b * a.q_heads + head) * a.q_len + row];
       m = st.x;
       ll = st.y;
-      if (half == 0) g.delta[at] = delta;
     }
   }
-  f32x16 acc[DP / 32];
+  f32x16 acc[DP / 32], pk[DP / 32];  // sums of dS k and of p k
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] = (f32x16)(0.f);
-  float flat_sum = 0.f;
-  float* my_sum = lds_sum + (2 * wave + half) * n_sum;
-  for (int i = threadIdx.x; i < 8 * n_sum; i += kAttnThreads) lds_sum[i] = 0.f;
+  for (int i = 0; i < DP / 32; ++i) acc[i] = pk[i] = (f32x16)(0.f);
+  float rest = 0.f;  // sum of dS: delta less dO . out
+  const f32x16 far_from = (f32x16)((bias ? bias[a.distances - 1] : 0.f) - m), minus_delta = (f32x16)(-delta);
 
   const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
   Stage ks, vs;
@@ -126,24 +129,29 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
     const int j0 = t * TK, j1 = j0 + TK - 1;
     const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
     if (seen) {
-      const bool flat = !bias || wc_lo - j1 >= a.distances - 1;
-      const float flat_bias = bias ? lb[kAttnRows - 32 - 32 * wave] : 0.f;
+      const bool far = !bias || wc_lo - j1 >= a.distances - 1;
       const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
                          wc_lo + 31 - j0 < a.window;
 #pragma unroll
       for (int s = 0; s < kSubs; ++s) {
-        f32x16 x, dp = (f32x16)(-delta);
-        if (flat) {
-          x = (f32x16)(flat_bias - m);
+        f32x16 x, dp;
+        auto products = [&](f32x16 from) {
+          x = F::mma(load_frag(lk + nat + 32 * s * LD), q[0], from);
+          dp = F::mma(load_frag(lv + nat + 32 * s * LD), go[0], minus_delta);
+#pragma unroll
+          for (int d = 1; d < kSteps; ++d) {
+            x = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x);
+            dp = F::mma(load_frag(lv + nat + 32 * s * LD + d * F::kStep), go[d], dp);
+          }
+        };
+        if (far) {
+          products(far_from);
         } else {
           const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
+          f32x16 near;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = from[8 * (i >> 2) + (i & 3)] - m;
-        }
-#pragma unroll
-        for (int d = 0; d < kSteps; ++d) {
-          x = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x);
-          dp = F::mma(load_frag(lv + nat + 32 * s * LD + d * F::kStep), go[d], dp);
+          for (int i = 0; i < 16; ++i) near[i] = from[8 * (i >> 2) + (i & 3)] - m;
+          products(near);
         }
         if (!whole) {
           uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
@@ -152,24 +160,21 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
           for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, -ll)) * dp[i];
-        if (n_sum) {
-          if (flat) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) flat_sum += x[i];
-          } else {
-            float* at = my_sum + (c - j0 - 32 * s - 4 * half + kSpare);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) lds_add(at - (8 * (i >> 2) + (i & 3)), x[i]);
-          }
+        for (int i = 0; i < 16; ++i) {
+          x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, -ll));
+          dp[i] *= x[i];
+          rest += dp[i];
         }
-        // dS takes the element type for the product with k
+        // p and dS take the element type for the products with k
 #pragma unroll
         for (int p = 0; p < 32 / F::kStep; ++p) {
-          const typename F::Frag pf = F::from_result(x, p);
+          const typename F::Frag pf = F::from_result(x, p), sf = F::from_result(dp, p);
 #pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt)
-            acc[dt] = F::mma(F::load_t(lk + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), pf, acc[dt]);
+          for (int dt = 0; dt < DP / 32; ++dt) {
+            const typename F::Frag kt = F::load_t(lk + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD);
+            acc[dt] = F::mma(kt, sf, acc[dt]);
+            pk[dt] = F::mma(kt, pf, pk[dt]);
+          }
         }
       }
     }
@@ -177,36 +182,90 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
     bits = bits_next;
     buf ^= 1;
   }
-  if (row < a.q_len)
-    store_result_row<T, DP>(static_cast<T*>(g.dq) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim, acc,
-                            a.scale, a.dim);
-  if (!n_sum) return;
-
-  // the block's bias gradient by bucket
-  for (int s = 32; s >= 1; s >>= 1) flat_sum += __shfl_xor(flat_sum, s);
-  __syncthreads();
-  if (lane_id() == 0) lds_bias[wave] = flat_sum;
-  for (int i = threadIdx.x; i < n_sum; i += kAttnThreads) {
-    float s = 0.f;
+  rest = sum_halves(rest);
+  if (row >= a.q_len) return;
+  if (half == 0) g.delta[((int64_t)b * a.q_heads + head) * a.q_len + row] = delta + rest;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += lds_sum[w * n_sum + i];
-    lds_sum[i] = s;
-  }
-  __syncthreads();
-  float* partial = g.bias_partial + (((int64_t)head * a.batch + b) * blocks_q + qb) * g.buckets;
-  const int sub = threadIdx.x & 7;
-  for (int k = threadIdx.x >> 3; k < g.buckets; k += kAttnThreads / 8) {
-    const int lo = k == 0 ? 0 : g.starts[k - 1];
-    const int hi = k == g.buckets - 1 ? n_sum - kSpare : g.starts[k];
-    float s = 0.f;
-    for (int d = lo + sub; d < hi; d += 8) s += lds_sum[d + kSpare];
-    for (int x = 4; x >= 1; x >>= 1) s += __shfl_xor(s, x);
-    if (k == g.buckets - 1) s += (lds_bias[0] + lds_bias[1]) + (lds_bias[2] + lds_bias[3]);
-    if (sub == 0) partial[k] = s;
-  }
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = __builtin_fmaf(-rest, pk[dt][i], acc[dt][i]);
+  store_result_row<T, DP>(static_cast<T*>(g.dq) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim, acc,
+                          a.scale, a.dim);
 }
 
-// ---------------------------------------------------------- keys: dk and dv --
+// ------------------------------------------------------ keys: dk, dv, bias --
+//
+// The bias gradient sums dS along diagonals (one distance each).  A product
+// tile is written to LDS skewed, so that a column holds one distance, and its
+// columns are summed by the lanes into four registers each (64 distances of
+// which a tile fills 63).  Along the walk the next tile's distances lie 32
+// further: half of the sums are complete, cross the lanes and are stored, the
+// other half moves down.  (One LDS addition per value instead cost 356 us
+// where the kernel's products cost 159.)  Tiles wholly in the last bucket
+// are summed into one register.
+
+struct DiagonalSums {
+  float* skew;   // [32][kSkew] of the wave; places outside the tile's band stay 0
+  float* sums;   // of the wave, by distance: sums[distance - shift + kSpare]
+  float acc[4];  // distances at - 31 + 4 (lane % 16) + i, rows lane / 16 + 4 k
+  float flat;
+  int at;        // distance of the tile's corner (row 0, column 0)
+  bool open;
+
+  __device__ __forceinline__ void reset() {
+    flat = 0.f;
+    open = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = 0.f;
+  }
+  // the 32 distances from `from` on, held by lanes 0 .. 7 of every 16
+  __device__ __forceinline__ void leave(int from) {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i]), __float_as_uint(acc[i]), false, false);
+      v[i] = sum_halves(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+    }
+    if (lane_id() < 8) *reinterpret_cast<f32x4*>(sums + (from & ~3) + kSpare + 4 * lane_id()) = v;
+  }
+  __device__ __forceinline__ void move_down() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // lane i takes lane i + 8 of its 16, zeros above
+      acc[i] = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(acc[i]), 0x108, 0xf, 0xf, true));
+  }
+  // both halves of what is open leave
+  __device__ __forceinline__ void close() {
+    if (!open) return;
+    leave(at - 31);
+    move_down();
+    leave(at + 1);
+    move_down();
+    open = false;
+  }
+  __device__ __forceinline__ void add(const f32x16& ds, int corner) {
+    if (open && corner == at + 32) {
+      leave(at - 31);
+      move_down();
+    } else {
+      close();
+    }
+    at = corner;
+    open = true;
+    // (row q, column n) -> skew[q][q - n + 31]
+    float* to = skew + 4 * (lane_id() >> 5) * (kSkew + 1) + 31 - (lane_id() & 31);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) to[(8 * (i >> 2) + (i & 3)) * (kSkew + 1)] = ds[i];
+    wave_sync();
+    const float* from = skew + (lane_id() >> 4) * kSkew + 4 * (lane_id() & 15);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(from + 4 * k * kSkew);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += v[i];
+    }
+    wave_sync();
+  }
+};
 
 // kFar: the pairs of the first tokens and the queries a window or more past
 // them.  Every query after a first token sees it, so a block of first tokens
@@ -223,6 +282,10 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   T* lds = reinterpret_cast<T*>(smem);                             // [2][Q, dO][TQ][LD]
   float* lds_row = reinterpret_cast<float*>(lds + 4 * TQ * LD);    // [2][m, log2 sum, delta][TQ]
   float* lds_bias = lds_row + 6 * TQ;                              // [2][kBias]
+  float* lds_skew = lds_bias + 2 * kBias;                          // [waves][32][kSkew], with a bias gradient
+  float* lds_sum = lds_skew + 4 * 32 * kSkew;                      // [waves][n_sum]
+  const int n_sum = g.bias_partial ? a.distances + 2 * kSpare : 0;  // a multiple of 4 from here on
+  const int n_pad = (n_sum + 3) & ~3;
 
   const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
   const int key_blocks = ((kFar ? a.sinks : a.k_len) + kAttnRows - 1) / kAttnRows;
@@ -239,7 +302,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   const int first = a.words ? a.first[b] : 0;
   const int sink_end = first + a.sinks < a.k_len ? first + a.sinks : a.k_len;
 
-  const int wave = threadIdx.x / kWave, l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
   const int k0 = (kFar ? first : 0) + kb * kAttnRows;
   const int k_end = kFar ? sink_end : a.k_len;
   const int jw = k0 + 32 * wave, j = jw + l32;
@@ -254,6 +317,45 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = (f32x16)(0.f);
+
+  // distances of a wave's tiles are alike modulo 32: stored from a multiple of 4
+  const int shift = (off - k0 + 1) & 3;
+  DiagonalSums diag{lds_skew + wave * 32 * kSkew, lds_sum + wave * n_pad, {}, 0.f, 0, false};
+  diag.reset();
+  if (n_sum) {
+    for (int i = threadIdx.x; i < 4 * 32 * kSkew; i += kAttnThreads) lds_skew[i] = 0.f;
+    for (int i = threadIdx.x; i < 4 * n_pad; i += kAttnThreads) lds_sum[i] = 0.f;
+  }
+  // The bias gradient of one head of the group, by bucket; sums start anew.
+  auto leave_head = [&](int hs) {
+    diag.close();
+    float flat = diag.flat;
+    for (int s = 32; s >= 1; s >>= 1) flat += __shfl_xor(flat, s);
+    __syncthreads();
+    if (lane_id() == 0) lds_skew[wave * 32 * kSkew + kSkew - 1] = flat;  // a place no tile fills
+    for (int i = threadIdx.x; i < n_pad; i += kAttnThreads)
+      lds_sum[i] = (lds_sum[i] + lds_sum[n_pad + i]) + (lds_sum[2 * n_pad + i] + lds_sum[3 * n_pad + i]);
+    __syncthreads();
+    const int64_t part = kFar ? g.bias_far + ((int64_t)b * g.far_chunks + chunk) * key_blocks + kb
+                              : (int64_t)b * key_blocks + kb;
+    float* partial = g.bias_partial + ((int64_t)(kv * share + hs) * g.bias_parts + part) * g.buckets;
+    const int sub = threadIdx.x & 7;
+    for (int k = threadIdx.x >> 3; k < g.buckets; k += kAttnThreads / 8) {
+      const int lo = k == 0 ? 0 : g.starts[k - 1];
+      const int hi = k == g.buckets - 1 ? a.distances + kSpare - 4 : g.starts[k];
+      float s = 0.f;
+      for (int d = lo + sub; d < hi; d += 8) s += lds_sum[d - shift + kSpare];
+      for (int x = 4; x >= 1; x >>= 1) s += __shfl_xor(s, x);
+      if (k == g.buckets - 1)
+        for (int w = 0; w < 4; ++w) s += lds_skew[w * 32 * kSkew + kSkew - 1];
+      if (sub == 0) partial[k] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < 4) lds_skew[threadIdx.x * 32 * kSkew + kSkew - 1] = 0.f;
+    for (int i = threadIdx.x; i < 4 * n_pad; i += kAttnThreads) lds_sum[i] = 0.f;
+    __syncthreads();
+    diag.reset();
+  };
 
   // query rows with a pair here
   int r_lo, r_hi;
@@ -310,6 +412,8 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   if (t_last < 0) hs = share;
   seek(hs, t, bits);
   if (hs < share) fetch(hs, t, bits);
+  else if (n_sum)
+    for (int i = 0; i < share; ++i) leave_head(i);
   int buf = 0;
   while (hs < share) {
     T* lq = lds + buf * 2 * TQ * LD;
@@ -332,12 +436,13 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
     const int c0 = t * TQ + off, c1 = c0 + TQ - 1;
     const bool seen = k_bits && (kFar ? c1 >= jw + a.window : c1 >= jw && c0 - (jw + 31) < a.window);
     if (seen) {
-      const bool flat = !a.bias || c0 - (jw + 31) >= a.distances - 1;
-      const float flat_bias = a.bias ? lb[kAttnRows - 32 - 32 * wave] : 0.f;
+      const float far_bias = a.bias ? lb[kAttnRows - 32 - 32 * wave + TQ - 32] : 0.f;
       const bool whole = k_bits == ~0u && (TQ == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) &&
                          (kFar ? c0 >= jw + 31 + a.window : c0 >= jw + 31 && c1 - jw < a.window);
 #pragma unroll
       for (int s = 0; s < kSubs; ++s) {
+        const int corner = c0 + 32 * s - jw;
+        const bool far = !a.bias || corner - 31 >= a.distances - 1;
         f32x16 x, dp;
         const float* rows = lr + 32 * s + 4 * half;
 #pragma unroll
@@ -345,9 +450,9 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
           x[i] = -rows[8 * (i >> 2) + (i & 3)];
           dp[i] = -rows[2 * TQ + 8 * (i >> 2) + (i & 3)];
         }
-        if (flat) {
+        if (far) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] += flat_bias;
+          for (int i = 0; i < 16; ++i) x[i] += far_bias;
         } else {
           const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
 #pragma unroll
@@ -379,6 +484,14 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= dp[i];
+        if (n_sum) {
+          if (far) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) diag.flat += x[i];
+          } else {
+            diag.add(x, corner - shift);
+          }
+        }
 #pragma unroll
         for (int p = 0; p < 32 / F::kStep; ++p) {
           const typename F::Frag sf = F::from_result(x, p);
@@ -388,6 +501,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
         }
       }
     }
+    if (n_sum && hs_next != hs) leave_head(hs);
     hs = hs_next;
     t = t_next;
     bits = bits_next;
@@ -429,7 +543,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
 
 struct BackwardLayout {
   size_t delta = 0, bias = 0, far = 0, bytes = 0;
-  int64_t bias_parts = 0;
+  int64_t bias_parts = 0, bias_far = 0;
   int32_t far_chunks = 0;
   explicit BackwardLayout(const mdl_attention& a) {
     auto take = [&](size_t n) {
@@ -438,14 +552,16 @@ struct BackwardLayout {
       return at;
     };
     delta = take((size_t)a.batch * a.q_heads * a.q_len * 4);
-    if (a.bias_table) {
-      bias_parts = a.batch * ((a.q_len + kAttnRows - 1) / kAttnRows);
-      bias = take((size_t)bias_parts * a.q_heads * a.num_buckets * 4);
-    }
     if (a.window > 0 && a.window < a.k_len && a.sinks > 0) {
       const int64_t sinks = a.sinks < a.k_len ? a.sinks : a.k_len;
       far_chunks = (int32_t)((a.q_len + kFarRows - 1) / kFarRows);
       far = take((size_t)a.batch * a.kv_heads * far_chunks * sinks * 2 * a.head_dim * 4);
+      bias_parts = a.batch * far_chunks * ((sinks + kAttnRows - 1) / kAttnRows);
+    }
+    if (a.bias_table) {
+      bias_far = a.batch * ((a.k_len + kAttnRows - 1) / kAttnRows);
+      bias_parts += bias_far;
+      bias = take((size_t)bias_parts * a.q_heads * a.num_buckets * 4);
     }
   }
 };
@@ -456,14 +572,14 @@ int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
   const size_t tiles = (size_t)4 * F::kTile * (DP + F::kPad) * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
   {
     const int64_t blocks = (int64_t)((a.q_len + kAttnRows - 1) / kAttnRows) * a.q_heads * a.batch;
-    const size_t lds = tiles + (g.bias_partial ? (size_t)8 * (a.distances + 2 * kSpare) * sizeof(float) : 0);
     const auto kernel = attention_grad_q_kernel<T, DP, kVec>;
     if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
-    if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
+    if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), tiles)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), tiles, s, a, g);
     MDL_CHECK_LAUNCH("attention_grad_q_kernel");
   }
-  const size_t lds = tiles + (size_t)6 * F::kTile * sizeof(float);
+  size_t lds = tiles + (size_t)6 * F::kTile * sizeof(float);
+  if (g.bias_partial) lds += (size_t)4 * (32 * kSkew + ((a.distances + 2 * kSpare + 3) & ~3)) * sizeof(float);
   if (g.far_partial) {
     const int64_t blocks =
         (int64_t)((a.sinks + kAttnRows - 1) / kAttnRows) * g.far_chunks * a.kv_heads * a.batch;
@@ -515,6 +631,8 @@ int mdl_attention_backward(const mdl_attention* a, const void* prepared, const m
   g.starts = a->bucket_starts;
   g.buckets = a->num_buckets;
   g.bias_partial = grads->grad_table ? reinterpret_cast<float*>(ws + lay.bias) : nullptr;
+  g.bias_parts = lay.bias_parts;
+  g.bias_far = lay.bias_far;
   g.far_partial = lay.far_chunks ? reinterpret_cast<float*>(ws + lay.far) : nullptr;
   g.far_chunks = lay.far_chunks;
   const int64_t e = a->dtype == MDL_BF16 ? 8 : 4;

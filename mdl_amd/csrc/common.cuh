@@ -428,6 +428,10 @@ __host__ __device__ __forceinline__ bool table_vec_of(uint64_t weight, int64_t d
 
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & (kWave - 1)); }
 
+// The wave's index in its block, known to the compiler to be one value per
+// wave (branches on it are scalar).
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)); }
+
 __device__ __forceinline__ float shfl_f(float v, int src) {
   return __int_as_float(__builtin_amdgcn_ds_bpermute(src << 2, __float_as_int(v)));
 }

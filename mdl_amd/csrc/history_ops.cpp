@@ -206,6 +206,7 @@ struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("mdl_hip::history_attention_backward", "")
                                .typed<decltype(attention_backward_cuda)>();
@@ -399,6 +400,7 @@ struct RelativeBias : public torch::autograd::Function<RelativeBias> {
     return call_relative_bias(table, starts, bidirectional, q_len, k_len);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("mdl_hip::relative_position_bias_backward", "")
                                .typed<decltype(relative_bias_grad_cuda)>();
@@ -557,6 +559,7 @@ struct BlockNorm : public torch::autograd::Function<BlockNorm> {
     const bool two = s[1].defined();
     const Tensor dy = two ? grads[0] : none, dh = grads[two ? 1 : 0];
     if (!dy.defined() && !dh.defined()) return {none, none, none, none, none, none, none};
+    at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("mdl_hip::block_norm_backward", "")
                                .typed<decltype(block_norm_backward_cuda)>();
