@@ -61,7 +61,9 @@ struct Frags<bf16_t> {
   static constexpr int kStep = 16;   // summed index per product
   static constexpr int kElems = 8;   // of it per lane
   static constexpr int kTile = 64;   // rows of a staged tile
-  static constexpr int kPad = 8;     // row padding in LDS (16 bytes: rows start 4 banks apart)
+  // Row padding in LDS, such that eight rows read in 16-byte pieces and four
+  // rows of 32 bytes read transposed both fall on different banks.
+  static constexpr int pad(int dp) { return dp == 64 ? 8 : 16; }
   typedef bf16x8 Frag;
 
   static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
@@ -93,7 +95,7 @@ struct Frags<float> {
   static constexpr int kStep = 8;
   static constexpr int kElems = 4;
   static constexpr int kTile = 32;
-  static constexpr int kPad = 4;
+  static constexpr int pad(int) { return 4; }
   typedef f32x4 Frag;
 
   static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
@@ -194,7 +196,7 @@ __device__ __forceinline__ void load_own_row(const T* row, bool live, int D,
 template <typename T, int DP, bool kVec>
 struct TileStage {
   using F = Frags<T>;
-  static constexpr int kLd = DP + F::kPad;
+  static constexpr int kLd = DP + F::pad(DP);
   static constexpr int kPieces = DP / F::kElems;  // per row
   static constexpr int kPer = F::kTile * kPieces / kAttnThreads;
   static_assert(F::kTile * kPieces % kAttnThreads == 0, "whole pieces per thread");

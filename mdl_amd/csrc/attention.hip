@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
 template <typename T, int DP>
 size_t forward_lds() {
   using F = Frags<T>;
-  return (size_t)4 * F::kTile * (DP + F::kPad) * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
+  return (size_t)4 * F::kTile * TileStage<T, DP, true>::kLd * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
 }
 
 template <typename T, int DP, bool kVec>

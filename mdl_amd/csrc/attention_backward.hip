@@ -37,7 +37,7 @@ struct GradCall {
 };
 
 constexpr int kSpare = 96;      // distances of one tile and wave past either end of the bias
-constexpr int kFarRows = 512;   // query rows of a block of the first tokens' far part
+constexpr int kFarRows = 256;   // query rows of a block of the first tokens' far part
 constexpr int kSkew = 64;       // diagonals of a 32x32 product tile, padded
 
 // ------------------------------------------------------ queries: dq, delta --
@@ -267,112 +267,174 @@ struct DiagonalSums {
   }
 };
 
-// kFar: the pairs of the first tokens and the queries a window or more past
-// them.  Every query after a first token sees it, so a block of first tokens
-// alone would walk the whole row while the others walk one window; these
-// pairs are cut into kFarRows query rows a block instead, whose parts the
-// block that owns the keys adds in order.
-template <typename T, int DP, bool kVec, bool kFar>
-__global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCall a, GradCall g) {
+// One 32x32 product tile: 32 queries (rows, staged in LDS) and the wave's 32
+// keys (columns, one per lane).
+template <typename T, int DP>
+struct KeyTile {
   using F = Frags<T>;
-  using Stage = TileStage<T, DP, kVec>;
-  constexpr int TQ = F::kTile, LD = Stage::kLd, kSteps = DP / F::kStep, kSubs = TQ / 32;
-  constexpr int kBias = kAttnRows + TQ;
-  extern __shared__ __align__(16) char smem[];
-  T* lds = reinterpret_cast<T*>(smem);                             // [2][Q, dO][TQ][LD]
-  float* lds_row = reinterpret_cast<float*>(lds + 4 * TQ * LD);    // [2][m, log2 sum, delta][TQ]
-  float* lds_bias = lds_row + 6 * TQ;                              // [2][kBias]
-  float* lds_skew = lds_bias + 2 * kBias;                          // [waves][32][kSkew], with a bias gradient
-  float* lds_sum = lds_skew + 4 * 32 * kSkew;                      // [waves][n_sum]
-  const int n_sum = g.bias_partial ? a.distances + 2 * kSpare : 0;  // a multiple of 4 from here on
-  const int n_pad = (n_sum + 3) & ~3;
-
-  const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
-  const int key_blocks = ((kFar ? a.sinks : a.k_len) + kAttnRows - 1) / kAttnRows;
-  int64_t id = xcd_block(blockIdx.x, gridDim.x);
-  const int kb = (int)(id % key_blocks);  // first keys first: without a window they walk the most tiles
-  id /= key_blocks;
-  int chunk = 0;
-  if (kFar) {
-    chunk = (int)(id % g.far_chunks);
-    id /= g.far_chunks;
-  }
-  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
-  const uint64_t* words = a.words ? a.words + (int64_t)b * a.words_row : nullptr;
-  const int first = a.words ? a.first[b] : 0;
-  const int sink_end = first + a.sinks < a.k_len ? first + a.sinks : a.k_len;
-
-  const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
-  const int k0 = (kFar ? first : 0) + kb * kAttnRows;
-  const int k_end = kFar ? sink_end : a.k_len;
-  const int jw = k0 + 32 * wave, j = jw + l32;
-  const uint32_t k_bits = columns32(a, words, jw) & low_bits(k_end - jw);
-  const bool live = (k_bits >> l32) & 1;
-
-  typename F::Frag kf[kSteps], vf[kSteps];
-  load_own_row<T, DP, kVec>(static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head + (int64_t)j * a.k_row, live,
-                            a.dim, kf);
-  load_own_row<T, DP, kVec>(static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head + (int64_t)j * a.v_row, live,
-                            a.dim, vf);
+  static constexpr int kSteps = DP / F::kStep;
+  typename F::Frag k[kSteps], v[kSteps];
   f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = (f32x16)(0.f);
 
-  // distances of a wave's tiles are alike modulo 32: stored from a multiple of 4
-  const int shift = (off - k0 + 1) & 3;
-  DiagonalSums diag{lds_skew + wave * 32 * kSkew, lds_sum + wave * n_pad, {}, 0.f, 0, false};
-  diag.reset();
-  if (n_sum) {
-    for (int i = threadIdx.x; i < 4 * 32 * kSkew; i += kAttnThreads) lds_skew[i] = 0.f;
-    for (int i = threadIdx.x; i < 4 * n_pad; i += kAttnThreads) lds_sum[i] = 0.f;
+  template <bool kVec>
+  __device__ __forceinline__ void open(const AttnCall& a, int b, int kv, int j, bool live) {
+    load_own_row<T, DP, kVec>(static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head + (int64_t)j * a.k_row, live,
+                              a.dim, k);
+    load_own_row<T, DP, kVec>(static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head + (int64_t)j * a.v_row, live,
+                              a.dim, v);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = (f32x16)(0.f);
   }
-  // The bias gradient of one head of the group, by bucket; sums start anew.
-  auto leave_head = [&](int hs) {
+
+  // Adds the tile to dk and dv; returns dS.  q, go: the 32 staged rows; rows:
+  // their -m, -log2 sum and -delta, pitch apart; near_bias: the pairs' biases
+  // by row (NULL: all far_bias); vis: the visible rows of the lane's key.
+  __device__ __forceinline__ f32x16 add(const T* q, const T* go, int LD, const float* rows, int pitch, float far_bias,
+                                        const float* near_bias, bool whole, uint32_t vis, float c2) {
+    const int l32 = lane_id() & 31, half = lane_id() >> 5;
+    const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
+    rows += 4 * half;
+    f32x16 x, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = rows[8 * (i >> 2) + (i & 3)];
+      dp[i] = rows[2 * pitch + 8 * (i >> 2) + (i & 3)];
+    }
+    if (near_bias) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] += near_bias[8 * (i >> 2) + (i & 3)];
+    } else if (far_bias != 0.f) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] += far_bias;
+    }
+#pragma unroll
+    for (int d = 0; d < kSteps; ++d) {
+      x = F::mma(load_frag(q + nat + d * F::kStep), k[d], x);
+      dp = F::mma(load_frag(go + nat + d * F::kStep), v[d], dp);
+    }
+    if (!whole) {
+      vis >>= 4 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], c2, rows[pitch + 8 * (i >> 2) + (i & 3)]));
+#pragma unroll
+    for (int p = 0; p < 32 / F::kStep; ++p) {
+      const typename F::Frag pf = F::from_result(x, p);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+        dv[dt] = F::mma(F::load_t(go + tr + F::kStep * p * LD + 32 * dt, LD), pf, dv[dt]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= dp[i];
+#pragma unroll
+    for (int p = 0; p < 32 / F::kStep; ++p) {
+      const typename F::Frag sf = F::from_result(x, p);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+        dk[dt] = F::mma(F::load_t(q + tr + F::kStep * p * LD + 32 * dt, LD), sf, dk[dt]);
+    }
+    return x;
+  }
+};
+
+// The bias gradient of a block, one head of its group at a time.
+struct BlockBias {
+  float *skew, *sums;  // [waves][32][kSkew], [waves][n_pad]
+  int n_pad, shift;    // distances of a wave's tiles are alike modulo 32: stored from a multiple of 4
+  DiagonalSums diag;
+
+  // any_corner: distance of any tile's corner
+  __device__ __forceinline__ void open(const AttnCall& a, float* lds, int any_corner) {
+    n_pad = (a.distances + 2 * kSpare + 3) & ~3;
+    skew = lds;
+    sums = lds + 4 * 32 * kSkew;
+    shift = (any_corner + 1) & 3;
+    diag.skew = skew + wave_id() * 32 * kSkew;
+    diag.sums = sums + wave_id() * n_pad;
+    diag.reset();
+    for (int i = threadIdx.x; i < 4 * 32 * kSkew; i += kAttnThreads) skew[i] = 0.f;
+    for (int i = threadIdx.x; i < 4 * n_pad; i += kAttnThreads) sums[i] = 0.f;
+    __syncthreads();
+  }
+  // Writes the head's sums by bucket and starts anew (every wave calls it).
+  __device__ __forceinline__ void leave(const AttnCall& a, const GradCall& g, int head, int64_t part) {
     diag.close();
     float flat = diag.flat;
     for (int s = 32; s >= 1; s >>= 1) flat += __shfl_xor(flat, s);
     __syncthreads();
-    if (lane_id() == 0) lds_skew[wave * 32 * kSkew + kSkew - 1] = flat;  // a place no tile fills
+    if (lane_id() == 0) diag.skew[kSkew - 1] = flat;  // a place no tile fills
     for (int i = threadIdx.x; i < n_pad; i += kAttnThreads)
-      lds_sum[i] = (lds_sum[i] + lds_sum[n_pad + i]) + (lds_sum[2 * n_pad + i] + lds_sum[3 * n_pad + i]);
+      sums[i] = (sums[i] + sums[n_pad + i]) + (sums[2 * n_pad + i] + sums[3 * n_pad + i]);
     __syncthreads();
-    const int64_t part = kFar ? g.bias_far + ((int64_t)b * g.far_chunks + chunk) * key_blocks + kb
-                              : (int64_t)b * key_blocks + kb;
-    float* partial = g.bias_partial + ((int64_t)(kv * share + hs) * g.bias_parts + part) * g.buckets;
+    float* partial = g.bias_partial + ((int64_t)head * g.bias_parts + part) * g.buckets;
     const int sub = threadIdx.x & 7;
     for (int k = threadIdx.x >> 3; k < g.buckets; k += kAttnThreads / 8) {
       const int lo = k == 0 ? 0 : g.starts[k - 1];
       const int hi = k == g.buckets - 1 ? a.distances + kSpare - 4 : g.starts[k];
       float s = 0.f;
-      for (int d = lo + sub; d < hi; d += 8) s += lds_sum[d - shift + kSpare];
+      for (int d = lo + sub; d < hi; d += 8) s += sums[d - shift + kSpare];
       for (int x = 4; x >= 1; x >>= 1) s += __shfl_xor(s, x);
       if (k == g.buckets - 1)
-        for (int w = 0; w < 4; ++w) s += lds_skew[w * 32 * kSkew + kSkew - 1];
+        for (int w = 0; w < 4; ++w) s += skew[w * 32 * kSkew + kSkew - 1];
       if (sub == 0) partial[k] = s;
     }
     __syncthreads();
-    if (threadIdx.x < 4) lds_skew[threadIdx.x * 32 * kSkew + kSkew - 1] = 0.f;
-    for (int i = threadIdx.x; i < 4 * n_pad; i += kAttnThreads) lds_sum[i] = 0.f;
+    if (lane_id() == 0) diag.skew[kSkew - 1] = 0.f;
+    for (int i = threadIdx.x; i < 4 * n_pad; i += kAttnThreads) sums[i] = 0.f;
     __syncthreads();
     diag.reset();
-  };
+  }
+  __device__ __forceinline__ void add(const f32x16& ds, int corner, bool far) {
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) diag.flat += ds[i];
+    } else {
+      diag.add(ds, corner - shift);
+    }
+  }
+};
+
+// The pairs within a window: 128 keys a block, 32 per wave.
+template <typename T, int DP, bool kVec>
+__global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCall a, GradCall g) {
+  using F = Frags<T>;
+  using Stage = TileStage<T, DP, kVec>;
+  constexpr int TQ = F::kTile, LD = Stage::kLd, kSubs = TQ / 32;
+  constexpr int kBias = kAttnRows + TQ;
+  extern __shared__ __align__(16) char smem[];
+  T* lds = reinterpret_cast<T*>(smem);                           // [2][Q, dO][TQ][LD]
+  float* lds_row = reinterpret_cast<float*>(lds + 4 * TQ * LD);  // [2][-m, -log2 sum, -delta][TQ]
+  float* lds_bias = lds_row + 6 * TQ;                            // [2][kBias]
+
+  const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
+  const int key_blocks = (a.k_len + kAttnRows - 1) / kAttnRows;
+  int64_t id = xcd_block(blockIdx.x, gridDim.x);
+  const int kb = (int)(id % key_blocks);  // first keys first: without a window they walk the most tiles
+  id /= key_blocks;
+  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
+  const uint64_t* words = a.words ? a.words + (int64_t)b * a.words_row : nullptr;
+
+  const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
+  const int k0 = kb * kAttnRows, k_end = a.k_len;
+  const int jw = k0 + 32 * wave, j = jw + l32;
+  const uint32_t k_bits = columns32(a, words, jw);
+  const bool live = (k_bits >> l32) & 1;
+
+  KeyTile<T, DP> tile;
+  tile.template open<kVec>(a, b, kv, j, live);
+  const bool want_bias = g.bias_partial != nullptr;
+  BlockBias sums;
+  if (want_bias) sums.open(a, lds_bias + 2 * kBias, off - k0);
+  const int64_t part = (int64_t)b * key_blocks + kb;
 
   // query rows with a pair here
-  int r_lo, r_hi;
-  if (kFar) {
-    r_lo = chunk * kFarRows;
-    r_hi = r_lo + kFarRows - 1;
-    if (r_lo < k0 + a.window - off) r_lo = k0 + a.window - off;
-  } else {
-    r_lo = k0 - off;
-    r_hi = (k_end < k0 + kAttnRows ? k_end : k0 + kAttnRows) - 1 + a.window - 1 - off;
-  }
+  int r_lo = k0 - off, r_hi = (k_end < k0 + kAttnRows ? k_end : k0 + kAttnRows) - 1 + a.window - 1 - off;
   if (r_lo < 0) r_lo = 0;
   if (r_hi > a.q_len - 1) r_hi = a.q_len - 1;
-  const int t_first = r_lo / TQ;
-  const int t_last = k0 < k_end && r_lo <= r_hi ? r_hi / TQ : -1;
+  const int t_first = r_lo / TQ, t_last = r_lo <= r_hi ? r_hi / TQ : -1;
 
-  const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
   Stage qs, gs;
   float2 stat_next = make_float2(0.f, INFINITY);
   float delta_next = 0.f, bias_next = 0.f;
@@ -381,7 +443,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
     if (TQ == 32) return (uint64_t)lo;
     return lo | (uint64_t)columns32(a, words, t * TQ + off + 32) << 32;
   };
-  // (head of the group, tile) from (share_, t) on with an unmasked query
+  // (head of the group, tile) from (hs, t) on with an unmasked query
   auto seek = [&](int& hs, int& t, uint64_t& bits) {
     for (; hs < share; ++hs, t = t_first)
       for (; t <= t_last; ++t) {
@@ -412,8 +474,8 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   if (t_last < 0) hs = share;
   seek(hs, t, bits);
   if (hs < share) fetch(hs, t, bits);
-  else if (n_sum)
-    for (int i = 0; i < share; ++i) leave_head(i);
+  else if (want_bias)
+    for (int i = 0; i < share; ++i) sums.leave(a, g, kv * share + i, part);
   int buf = 0;
   while (hs < share) {
     T* lq = lds + buf * 2 * TQ * LD;
@@ -423,9 +485,9 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
     qs.store(lq);
     gs.store(lg);
     if (threadIdx.x < TQ) {
-      lr[threadIdx.x] = stat_next.x;
-      lr[TQ + threadIdx.x] = stat_next.y;
-      lr[2 * TQ + threadIdx.x] = delta_next;
+      lr[threadIdx.x] = -stat_next.x;
+      lr[TQ + threadIdx.x] = -stat_next.y;
+      lr[2 * TQ + threadIdx.x] = -delta_next;
     }
     if (a.bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
     int hs_next = hs, t_next = t + 1;
@@ -434,109 +496,183 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
     __syncthreads();
 
     const int c0 = t * TQ + off, c1 = c0 + TQ - 1;
-    const bool seen = k_bits && (kFar ? c1 >= jw + a.window : c1 >= jw && c0 - (jw + 31) < a.window);
+    const bool seen = k_bits && c1 >= jw && c0 - (jw + 31) < a.window;
     if (seen) {
+      // of the tile's largest distance: the far bias if any of its products is far
       const float far_bias = a.bias ? lb[kAttnRows - 32 - 32 * wave + TQ - 32] : 0.f;
-      const bool whole = k_bits == ~0u && (TQ == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) &&
-                         (kFar ? c0 >= jw + 31 + a.window : c0 >= jw + 31 && c1 - jw < a.window);
+      const bool whole = k_bits == ~0u && (TQ == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && c0 >= jw + 31 &&
+                         c1 - jw < a.window;
 #pragma unroll
       for (int s = 0; s < kSubs; ++s) {
-        const int corner = c0 + 32 * s - jw;
+        const int col = c0 + 32 * s, corner = col - jw;
         const bool far = !a.bias || corner - 31 >= a.distances - 1;
-        f32x16 x, dp;
-        const float* rows = lr + 32 * s + 4 * half;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] = -rows[8 * (i >> 2) + (i & 3)];
-          dp[i] = -rows[2 * TQ + 8 * (i >> 2) + (i & 3)];
-        }
-        if (far) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] += far_bias;
-        } else {
-          const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] += from[8 * (i >> 2) + (i & 3)];
-        }
-#pragma unroll
-        for (int d = 0; d < kSteps; ++d) {
-          x = F::mma(load_frag(lq + nat + 32 * s * LD + d * F::kStep), kf[d], x);
-          dp = F::mma(load_frag(lg + nat + 32 * s * LD + d * F::kStep), vf[d], dp);
-        }
-        if (!whole) {
-          const int col = c0 + 32 * s;
-          uint32_t vis = ~low_bits((kFar ? j + a.window : j) - col);
-          if (!kFar) vis &= low_bits(j + a.window - col);
-          vis = live ? vis & (uint32_t)(bits >> (32 * s)) : 0u;
-          vis >>= 4 * half;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, -rows[TQ + 8 * (i >> 2) + (i & 3)]));
-#pragma unroll
-        for (int p = 0; p < 32 / F::kStep; ++p) {
-          const typename F::Frag pf = F::from_result(x, p);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt)
-            dv[dt] = F::mma(F::load_t(lg + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), pf, dv[dt]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= dp[i];
-        if (n_sum) {
-          if (far) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) diag.flat += x[i];
-          } else {
-            diag.add(x, corner - shift);
-          }
-        }
-#pragma unroll
-        for (int p = 0; p < 32 / F::kStep; ++p) {
-          const typename F::Frag sf = F::from_result(x, p);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt)
-            dk[dt] = F::mma(F::load_t(lq + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), sf, dk[dt]);
-        }
+        uint32_t vis = 0;
+        if (!whole)
+          vis = live ? ~low_bits(j - col) & low_bits(j + a.window - col) & (uint32_t)(bits >> (32 * s)) : 0u;
+        const f32x16 ds =
+            tile.add(lq + 32 * s * LD, lg + 32 * s * LD, LD, lr + 32 * s, TQ, far_bias,
+                     far ? nullptr : lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half), whole, vis, a.c2);
+        if (want_bias) sums.add(ds, corner, far);
       }
     }
-    if (n_sum && hs_next != hs) leave_head(hs);
+    if (want_bias && hs_next != hs) sums.leave(a, g, kv * share + hs, part);
     hs = hs_next;
     t = t_next;
     bits = bits_next;
     buf ^= 1;
   }
 
-  if (kFar) {
-    if (j < k_end) {
-      float* part = g.far_partial +
-                    (((((int64_t)b * a.kv_heads + kv) * g.far_chunks + chunk) * a.sinks + (j - first)) * 2) * a.dim;
-      store_result_row<float, DP>(part, dk, 1.f, a.dim);
-      store_result_row<float, DP>(part + a.dim, dv, 1.f, a.dim);
-    }
-    return;
-  }
   if (j >= a.k_len) return;
-  if (g.far_partial && j >= first && j < sink_end) {
-    for (int n = 0; n < g.far_chunks; ++n) {
-      const float* part =
-          g.far_partial + (((((int64_t)b * a.kv_heads + kv) * g.far_chunks + n) * a.sinks + (j - first)) * 2) * a.dim;
+  if (g.far_partial) {
+    const int first = a.words ? a.first[b] : 0;
+    if (j >= first && j - first < a.sinks) {
+#pragma unroll 2
+      for (int n = 0; n < g.far_chunks; ++n) {
+        const float* far =
+            g.far_partial + (((((int64_t)b * a.kv_heads + kv) * g.far_chunks + n) * a.sinks + (j - first)) * 2) * a.dim;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = 32 * dt + result_row(i);
+            if (d < a.dim) {
+              tile.dk[dt][i] += far[d];
+              tile.dv[dt][i] += far[a.dim + d];
+            }
+          }
+      }
+    }
+  }
+  const int64_t at = (((int64_t)b * a.k_len + j) * a.kv_heads + kv) * a.dim;
+  store_result_row<T, DP>(static_cast<T*>(g.dk) + at, tile.dk, a.scale, a.dim);
+  store_result_row<T, DP>(static_cast<T*>(g.dv) + at, tile.dv, 1.f, a.dim);
+}
+
+// Waves of a block that walk: those whose staged rows fit LDS beside the bias.
+template <typename T, int DP>
+__host__ __device__ constexpr int far_waves() { return sizeof(T) == 4 && DP == 128 ? 2 : 4; }
+
+// The pairs of the first tokens and the queries a window or more past them.
+// Every query after a first token sees it, so a block that owned it whole
+// would walk the row while the others walk one window: these pairs are cut
+// into kFarRows query rows a block, whose parts the block that owns the keys
+// adds in order.  A block has 32 first tokens; its waves take 32 query rows
+// each in turn, staged in LDS of their own (no barrier in the walk).
+template <typename T, int DP, bool kVec>
+__global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCall a, GradCall g) {
+  using F = Frags<T>;
+  constexpr int LD = TileStage<T, DP, kVec>::kLd, kPieces = DP / F::kElems, kPer = 32 * kPieces / kWave;
+  constexpr int kBias = 64, kWalk = far_waves<T, DP>();
+  extern __shared__ __align__(16) char smem[];
+  const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
+  T* lq = reinterpret_cast<T*>(smem) + wave * 64 * LD;  // of the wave: [Q, dO][32][LD]
+  T* lg = lq + 32 * LD;
+  float* lr = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + kWalk * 64 * LD) + wave * (96 + kBias);
+  float* lb = lr + 96;
+  float* joined = reinterpret_cast<float*>(smem);  // [dk, dv][32][dim], after the walk
+
+  const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
+  const int key_blocks = (a.sinks + 31) / 32;
+  int64_t id = xcd_block(blockIdx.x, gridDim.x);
+  const int kb = (int)(id % key_blocks);
+  id /= key_blocks;
+  const int chunk = (int)(id % g.far_chunks);
+  id /= g.far_chunks;
+  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
+  const uint64_t* words = a.words ? a.words + (int64_t)b * a.words_row : nullptr;
+  const int first = a.words ? a.first[b] : 0;
+  const int k_end = first + a.sinks < a.k_len ? first + a.sinks : a.k_len;
+  const int k0 = first + 32 * kb, j = k0 + l32;
+  const uint32_t k_bits = columns32(a, words, k0) & low_bits(k_end - k0);
+  const bool live = (k_bits >> l32) & 1;
+
+  KeyTile<T, DP> tile;
+  tile.template open<kVec>(a, b, kv, j, live);
+  const bool want_bias = g.bias_partial != nullptr;
+  BlockBias sums;
+  if (want_bias)
+    sums.open(a, reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + kWalk * 64 * LD) + kWalk * (96 + kBias), off - k0);
+  const int64_t part = g.bias_far + ((int64_t)b * g.far_chunks + chunk) * key_blocks + kb;
+
+  const int r_first = chunk * kFarRows, r_last = r_first + kFarRows < a.q_len ? r_first + kFarRows : a.q_len;
+  for (int hs = 0; hs < share; ++hs) {
+    const int head = kv * share + hs;
+    const float far_bias = a.bias ? a.bias[(int64_t)head * a.distances + a.distances - 1] : 0.f;
+    const T* qp = static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head;
+    const T* gp = static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head;
+    for (int r0 = r_first + 32 * wave; wave < kWalk && r0 < r_last; r0 += 32 * kWalk) {
+      const int col = r0 + off;
+      const uint32_t bits = columns32(a, words, col);
+      if (!k_bits || !bits || col + 31 < k0 + a.window) continue;
+      typename F::Frag qr[kPer], gr[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = i * kWave + lane_id(), row = at / kPieces, d = at % kPieces * F::kElems;
+        qr[i] = gr[i] = {};
+        if ((bits >> row) & 1) {
+          qr[i] = load_row<T, kVec>(qp + (int64_t)(r0 + row) * a.q_row, d, a.dim);
+          gr[i] = load_row<T, kVec>(gp + (int64_t)(r0 + row) * g.g_row, d, a.dim);
+        }
+      }
+      float2 st = make_float2(0.f, INFINITY);
+      float delta = 0.f;
+      if (r0 + l32 < a.q_len) {
+        const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + r0 + l32;
+        st = g.stats[at];
+        delta = g.delta[at];
+      }
+      const int corner = col - k0;
+      const bool far = !a.bias || corner - 31 >= a.distances - 1;
+      float near = 0.f;
+      if (!far) {
+        // lb[i]: distance corner - 31 + i
+        int d = corner - 31 + lane_id();
+        d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
+        near = a.bias[(int64_t)head * a.distances + d];
+      }
+      wave_sync();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = i * kWave + lane_id();
+        *reinterpret_cast<typename F::Frag*>(lq + at / kPieces * LD + at % kPieces * F::kElems) = qr[i];
+        *reinterpret_cast<typename F::Frag*>(lg + at / kPieces * LD + at % kPieces * F::kElems) = gr[i];
+      }
+      if (half == 0) {
+        lr[l32] = -st.x;
+        lr[32 + l32] = -st.y;
+        lr[64 + l32] = -delta;
+      }
+      if (!far) lb[lane_id()] = near;
+      wave_sync();
+      const bool whole = k_bits == ~0u && bits == ~0u && corner - 31 >= a.window;
+      const uint32_t vis = live ? ~low_bits(j + a.window - col) & bits : 0u;
+      const f32x16 ds =
+          tile.add(lq, lg, LD, lr, 32, far_bias, far ? nullptr : lb + 31 - l32 + 4 * half, whole, vis, a.c2);
+      if (want_bias) sums.add(ds, corner, far);
+    }
+    if (want_bias) sums.leave(a, g, head, part);
+  }
+
+  // the waves' sums, added in order
+  for (int w = 0; w < kWalk; ++w) {
+    __syncthreads();
+    if (wave == w) {
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int d = 32 * dt + result_row(i);
-          if (d < a.dim) {
-            dk[dt][i] += part[d];
-            dv[dt][i] += part[a.dim + d];
-          }
+          float* at = joined + (32 * dt + result_row(i)) * 32 + l32;
+          at[0] = (w ? at[0] : 0.f) + tile.dk[dt][i];
+          at[DP * 32] = (w ? at[DP * 32] : 0.f) + tile.dv[dt][i];
         }
     }
   }
-  const int64_t at = (((int64_t)b * a.k_len + j) * a.kv_heads + kv) * a.dim;
-  store_result_row<T, DP>(static_cast<T*>(g.dk) + at, dk, a.scale, a.dim);
-  store_result_row<T, DP>(static_cast<T*>(g.dv) + at, dv, 1.f, a.dim);
+  __syncthreads();
+  float* to = g.far_partial + ((((int64_t)b * a.kv_heads + kv) * g.far_chunks + chunk) * a.sinks + 32 * kb) * 2 * a.dim;
+  for (int i = threadIdx.x; i < 32 * 2 * a.dim; i += kAttnThreads) {
+    const int key = i / (2 * a.dim), which = i / a.dim & 1, d = i % a.dim;
+    if (32 * kb + key < a.sinks) to[(int64_t)key * 2 * a.dim + which * a.dim + d] = joined[which * DP * 32 + d * 32 + key];
+  }
 }
 
 // ---------------------------------------------------------------- host side --
@@ -556,7 +692,7 @@ struct BackwardLayout {
       const int64_t sinks = a.sinks < a.k_len ? a.sinks : a.k_len;
       far_chunks = (int32_t)((a.q_len + kFarRows - 1) / kFarRows);
       far = take((size_t)a.batch * a.kv_heads * far_chunks * sinks * 2 * a.head_dim * 4);
-      bias_parts = a.batch * far_chunks * ((sinks + kAttnRows - 1) / kAttnRows);
+      bias_parts = a.batch * far_chunks * ((sinks + 31) / 32);
     }
     if (a.bias_table) {
       bias_far = a.batch * ((a.k_len + kAttnRows - 1) / kAttnRows);
@@ -569,7 +705,7 @@ struct BackwardLayout {
 template <typename T, int DP, bool kVec>
 int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
   using F = Frags<T>;
-  const size_t tiles = (size_t)4 * F::kTile * (DP + F::kPad) * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
+  const size_t tiles = (size_t)4 * F::kTile * TileStage<T, DP, true>::kLd * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
   {
     const int64_t blocks = (int64_t)((a.q_len + kAttnRows - 1) / kAttnRows) * a.q_heads * a.batch;
     const auto kernel = attention_grad_q_kernel<T, DP, kVec>;
@@ -578,19 +714,23 @@ int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), tiles, s, a, g);
     MDL_CHECK_LAUNCH("attention_grad_q_kernel");
   }
-  size_t lds = tiles + (size_t)6 * F::kTile * sizeof(float);
-  if (g.bias_partial) lds += (size_t)4 * (32 * kSkew + ((a.distances + 2 * kSpare + 3) & ~3)) * sizeof(float);
+  const size_t bias_lds =
+      g.bias_partial ? (size_t)4 * (32 * kSkew + ((a.distances + 2 * kSpare + 3) & ~3)) * sizeof(float) : 0;
   if (g.far_partial) {
-    const int64_t blocks =
-        (int64_t)((a.sinks + kAttnRows - 1) / kAttnRows) * g.far_chunks * a.kv_heads * a.batch;
-    const auto kernel = attention_grad_kv_kernel<T, DP, kVec, true>;
+    const int64_t blocks = (int64_t)((a.sinks + 31) / 32) * g.far_chunks * a.kv_heads * a.batch;
+    const size_t walk =
+        far_waves<T, DP>() * ((size_t)64 * TileStage<T, DP, true>::kLd * sizeof(T) + (96 + 64) * sizeof(float)) + bias_lds;
+    const size_t join = (size_t)2 * DP * 32 * sizeof(float);
+    const size_t lds = walk > join ? walk : join;
+    const auto kernel = attention_grad_far_kernel<T, DP, kVec>;
     if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
     if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
-    MDL_CHECK_LAUNCH("attention_grad_kv_kernel");
+    MDL_CHECK_LAUNCH("attention_grad_far_kernel");
   }
+  const size_t lds = tiles + (size_t)6 * F::kTile * sizeof(float) + bias_lds;
   const int64_t blocks = (int64_t)((a.k_len + kAttnRows - 1) / kAttnRows) * a.kv_heads * a.batch;
-  const auto kernel = attention_grad_kv_kernel<T, DP, kVec, false>;
+  const auto kernel = attention_grad_kv_kernel<T, DP, kVec>;
   if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
