@@ -698,7 +698,7 @@ int mdl_attention_prepare(const mdl_attention* call, void* prepared, size_t prep
 
 /* out: [batch, q_len, q_heads, head_dim] contiguous (dtype).  stats (NULL
  * without a backward): float [batch, q_heads, q_len, 2], each row's largest
- * score divided by scale and log2 of its softmax sum. */
+ * score divided by scale and log2 of its softmax sum, both negated. */
 int mdl_attention_forward(const mdl_attention* call, const void* prepared, void* out, float* stats, void* stream);
 
 /*

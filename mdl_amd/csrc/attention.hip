@@ -40,7 +40,7 @@ struct PrepareCall {
   const void* table;
   const int32_t* starts;
   uint64_t* words;
-  int32_t* first;
+  int2* bounds;
   float* bias;
   int64_t words_row;
   int32_t batch, k_len, heads, buckets, distances;
@@ -53,29 +53,42 @@ __global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
   int64_t block = blockIdx.x;
   if (a.mask) {
     if (block < a.batch) {
-      __shared__ int firsts[4];
+      __shared__ int firsts[4], lasts[4];
       const uint8_t* row = a.mask + block * a.mask_row;
       uint64_t* words = a.words + block * a.words_row;
-      int first = a.k_len;
+      int first = a.k_len, last = -1;
+#pragma unroll 4
       for (int w = wave; w < a.words_row; w += 4) {
         const int col = 64 * w + lane_id();
         const uint64_t word = __ballot(col < a.k_len && row[col] != 0);
-        if (word && first == a.k_len) first = 64 * w + __builtin_ctzll(word);
+        if (word) {
+          if (first == a.k_len) first = 64 * w + __builtin_ctzll(word);
+          last = 64 * w + 63 - __builtin_clzll(word);
+        }
         if (lane_id() == 0) words[w] = word;
       }
-      if (lane_id() == 0) firsts[wave] = first;
+      if (lane_id() == 0) {
+        firsts[wave] = first;
+        lasts[wave] = last;
+      }
       __syncthreads();
       if (threadIdx.x == 0) {
-        for (int i = 1; i < 4; ++i) first = firsts[i] < first ? firsts[i] : first;
-        a.first[block] = first;
+        for (int i = 1; i < 4; ++i) {
+          first = firsts[i] < first ? firsts[i] : first;
+          last = lasts[i] > last ? lasts[i] : last;
+        }
+        a.bounds[block] = make_int2(first, last);
       }
       return;
     }
     block -= a.batch;
   }
   const int64_t i = block * 256 + threadIdx.x;
-  if (i >= (int64_t)a.heads * a.distances) return;
-  const int h = (int)(i / a.distances), d = (int)(i % a.distances);
+  const int per_head = a.distances + 2 * kBiasEdge;
+  if (!a.bias || i >= (int64_t)a.heads * per_head) return;
+  const int h = (int)(i / per_head);
+  int d = (int)(i % per_head) - kBiasEdge;
+  d = d < 0 ? 0 : d;
   const int64_t at = (int64_t)bucket_of_distance(a.starts, a.buckets, d) * a.heads + h;
   const float v = a.table_f32 ? table_value(static_cast<const float*>(a.table) + at)
                               : table_value(static_cast<const bf16_t*>(a.table) + at);
@@ -91,35 +104,41 @@ __global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
 // (p stays below 2^8): most tiles then skip the rescaling of out.
 constexpr float kLazyRaise = 8.f;
 
+// Two waves more than the two that most registers would allow hide the
+// latencies of bf16's narrow tiles better than reading ahead.
+template <typename T, int DP>
+constexpr int forward_waves() { return sizeof(T) == 2 && DP <= 64 ? 3 : 1; }
+
 template <typename T, int DP, bool kVec>
-__global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCall a, T* out, float2* stats) {
+__global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attention_forward_kernel(AttnCall a, T* out,
+                                                                                                 float2* stats) {
   using F = Frags<T>;
   using Stage = TileStage<T, DP, kVec>;
-  constexpr int TK = F::kTile, LD = Stage::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;
-  constexpr int kBias = kAttnRows + TK;  // distances of a block and a tile
+  constexpr int TK = F::kTile, LD = Tile<T, DP>::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;
+  constexpr int kStages = tile_stages<T, DP, kVec>();
   extern __shared__ __align__(16) char smem[];
-  T* lds = reinterpret_cast<T*>(smem);                     // [2][K, V][TK][LD]
-  float* lds_bias = reinterpret_cast<float*>(lds + 4 * TK * LD);  // [2][kBias]
+  T* lds = reinterpret_cast<T*>(smem);                                       // [stages][K, V][TK][LD]
+  float* lds_bias = reinterpret_cast<float*>(lds + kStages * 2 * TK * LD);  // [stages][kBiasSpan]
 
-  const int blocks_q = (a.q_len + kAttnRows - 1) / kAttnRows;
-  int64_t id = xcd_block(blockIdx.x, gridDim.x);
-  // last rows first: without a window they walk the most tiles
-  const int qb = blocks_q - 1 - (int)(id % blocks_q);
-  id /= blocks_q;
-  const int head = (int)(id % a.q_heads), b = (int)(id / a.q_heads);
+  int unit, inner;
+  const BlockOrder order = query_blocks(a);
+  if (!order.place(blockIdx.x, &unit, &inner)) return;
+  const int qb = order.per_unit - 1 - inner;  // last rows first: without a window they walk the most tiles
+  const int b = unit / a.q_heads, head = unit - b * a.q_heads;
   const int kv = head / (a.q_heads / a.kv_heads);
   const T* kp = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
-  const float* bias = a.bias ? a.bias + (int64_t)head * a.distances : nullptr;
+  const float* bias = a.bias ? head_bias(a, head) : nullptr;
 
   const int off = a.k_len - a.q_len;
   const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
   const int r0 = qb * kAttnRows;
   const int r_end = r0 + kAttnRows < a.q_len ? r0 + kAttnRows : a.q_len;
   const int row = r0 + 32 * wave + l32, c = row + off;
-  KeyWalk walk(a, b, TK, r0 + off, r_end - 1 + off);
+  const RowMask mask(a, b);
+  const KeyWalk walk(a, mask, TK, r0 + off, r_end - 1 + off);
   const int wc_lo = r0 + 32 * wave + off;  // the wave's columns
-  const uint32_t q_bits = wc_lo - off < a.q_len ? columns32(a, walk.words, wc_lo) : 0;
+  const uint32_t q_bits = mask.bits32(wc_lo);
   const bool live = (q_bits >> l32) & 1;
 
   typename F::Frag q[kSteps];
@@ -130,106 +149,94 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
   for (int i = 0; i < DP / 32; ++i) acc[i] = (f32x16)(0.f);
   float m = kNoScore, mneg = -(kNoScore * a.c2), l = 0.f;
   const float lazy = kLazyRaise / a.c2;
+  const f32x16 far_bias = (f32x16)(bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f);
 
-  const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
-  const f32x16 far_bias = (f32x16)(bias ? bias[a.distances - 1] : 0.f);
+  const Tile<T, DP> read;
   Stage ks, vs;
-  float bias_next = 0.f;
-  auto fetch = [&](int t, uint64_t bits) {
-    ks.load(kp, a.k_row, t * TK, bits, a.dim);
-    vs.load(vp, a.v_row, t * TK, bits, a.dim);
-    if (bias && threadIdx.x < kBias) {
-      // lds_bias[i]: the distance of query i' and key k' with k' - i' = i - (rows - 1)
-      int d = r0 + off - t * TK + kAttnRows - 1 - (int)threadIdx.x;
-      d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
-      bias_next = bias[d];
-    }
+  auto fetch = [&](int i, int slot) {
+    const int j0 = walk.tile_at(i) * TK;
+    const uint64_t bits = mask.bits<TK>(j0);
+    T* to = lds + slot * 2 * TK * LD;
+    ks.fetch(to, kp, a.k_row, j0, bits, a.dim);
+    vs.fetch(to + TK * LD, vp, a.v_row, j0, bits, a.dim);
+    // lds_bias[i]: distance i + that of the block's first query and the tile's last key
+    if (bias)
+      copy4_to_lds(lds_bias + slot * kBiasSpan + wave * kWave, bias + bias_at(a, r0 + off - j0 - (TK - 1)) + threadIdx.x);
   };
-  uint64_t bits = 0, bits_next = 0;
-  int t = walk.begin(a, &bits);
-  if (t <= walk.last_tile) fetch(t, bits);
-  int buf = 0;
-  while (t <= walk.last_tile) {
-    T* lk = lds + buf * 2 * TK * LD;
-    T* lv = lk + TK * LD;
-    float* lb = lds_bias + buf * kBias;
-    ks.store(lk);
-    vs.store(lv);
-    if (bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
-    const int t_next = walk.seek(a, t + 1, &bits_next);
-    if (t_next <= walk.last_tile) fetch(t_next, bits_next);
-    __syncthreads();
-
-    const int j0 = t * TK, j1 = j0 + TK - 1;
+  auto settle = [&](int slot) {
+    ks.settle(lds + slot * 2 * TK * LD);
+    vs.settle(lds + slot * 2 * TK * LD + TK * LD);
+  };
+  auto work = [&](int i, int slot) {
+    const T* lk = lds + slot * 2 * TK * LD;
+    const T* lv = lk + TK * LD;
+    const int j0 = walk.tile_at(i) * TK, j1 = j0 + TK - 1;
     const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
-    if (seen) {
-      f32x16 x[kSubs];
-      auto products = [&](int s, f32x16 from) {
-        x[s] = F::mma(load_frag(lk + nat + 32 * s * LD), q[0], from);
-#pragma unroll
-        for (int d = 1; d < kSteps; ++d) x[s] = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x[s]);
-      };
-      // distances of the wave and the tile all in the last bucket, or none told apart
-      if (!bias || wc_lo - j1 >= a.distances - 1) {
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s) products(s, far_bias);
-      } else {
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s) {
-          const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
-          f32x16 near;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) near[i] = from[8 * (i >> 2) + (i & 3)];
-          products(s, near);
-        }
-      }
-      const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
-                         wc_lo + 31 - j0 < a.window;
-      if (!whole) {
-#pragma unroll
-        for (int s = 0; s < kSubs; ++s) {
-          uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
-          vis >>= 4 * half;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[s][i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[s][i], -INFINITY);
-        }
-      }
-      float top = x[0][0];
-#pragma unroll
-      for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, x[s][i]);
-      top = max_halves(top);
-      if (__any(top > m + lazy)) {
-        const float up = fmaxf(m, top);
-        const float shrink = exp2_fast((m - up) * a.c2);
-        m = up;
-        mneg = -(m * a.c2);
-        l *= shrink;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) acc[i] *= shrink;
-      }
+    if (!seen) return;
+    const uint64_t bits = mask.bits<TK>(j0);
+    f32x16 x[kSubs];
+    // distances of the wave and the tile all in the last bucket, or none told apart
+    const bool far = !bias || wc_lo - j1 >= a.distances - 1;
+    if (!far) {
 #pragma unroll
       for (int s = 0; s < kSubs; ++s) {
+        const float* from = lds_bias + slot * kBiasSpan + (32 * wave + l32 + TK - 1 - 32 * s - 4 * half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[s][i] = exp2_fast(__builtin_fmaf(x[s][i], a.c2, mneg));
-          l += x[s][i];
-        }
-        // the weights take the element type for the second product; their sum does not
-#pragma unroll
-        for (int p = 0; p < 32 / F::kStep; ++p) {
-          const typename F::Frag pf = F::from_result(x[s], p);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt)
-            acc[dt] = F::mma(F::load_t(lv + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD), pf, acc[dt]);
-        }
+        for (int i = 0; i < 16; ++i) x[s][i] = from[-(8 * (i >> 2) + (i & 3))];
       }
     }
-    t = t_next;
-    bits = bits_next;
-    buf ^= 1;
-  }
+#pragma unroll
+    for (int s = 0; s < kSubs; ++s) {
+      const NatFrags<T, DP> k(read, lk, s);
+      if constexpr (DP > 64) reads_first<T>();
+      x[s] = far ? k.times(q, far_bias) : k.times(q, x[s]);
+    }
+    const TrFrags<T, DP> v0(read, lv, 0);
+    const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
+                       wc_lo + 31 - j0 < a.window;
+    if (!whole) {
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) {
+        uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
+        vis >>= 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[s][i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[s][i], -INFINITY);
+      }
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[s][i]);
+    top = max_halves(top);
+    if (__any(top > m + lazy)) {
+      const float up = fmaxf(m, top);
+      const float shrink = exp2_fast((m - up) * a.c2);
+      m = up;
+      mneg = -(m * a.c2);
+      l *= shrink;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= shrink;
+    }
+    // the weights take the element type for the second product; their sum does not
+    auto weigh = [&](f32x16& w) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        w[i] = exp2_fast(__builtin_fmaf(w[i], a.c2, mneg));
+        l += w[i];
+      }
+    };
+    weigh(x[0]);
+    if constexpr (kSubs == 2) {
+      const TrFrags<T, DP> v1(read, lv, 1);
+      v0.times(x[0], acc);
+      weigh(x[1]);
+      v1.times(x[1], acc);
+    } else {
+      v0.times(x[0], acc);
+    }
+  };
+  walk_tiles<kStages, 2 * Stage::kPer, Stage::kDirect>(walk.tiles, bias != nullptr, fetch, settle, work);
 
   l = sum_halves(l);
   if (row < a.q_len) {
@@ -237,24 +244,23 @@ __global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCal
     const float inv = l > 0.f ? 1.f / l : 0.f;
     store_result_row<T, DP>(out + at, acc, inv, a.dim);
     if (stats && half == 0) {
-      // log2 of the sum at the unrounded c2 m; +inf makes every weight of an empty row 0
-      const float ll = l > 0.f ? log2f(l) - __builtin_fmaf(m, a.c2, mneg) : INFINITY;
-      stats[((int64_t)b * a.q_heads + head) * a.q_len + row] = make_float2(l > 0.f ? m : 0.f, ll);
+      // -m and -log2 of the sum at the unrounded c2 m; -inf makes every weight of an empty row 0
+      const float ll = l > 0.f ? __builtin_fmaf(m, a.c2, mneg) - log2f(l) : -INFINITY;
+      stats[((int64_t)b * a.q_heads + head) * a.q_len + row] = make_float2(l > 0.f ? -m : 0.f, ll);
     }
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kVec>
 size_t forward_lds() {
-  using F = Frags<T>;
-  return (size_t)4 * F::kTile * TileStage<T, DP, true>::kLd * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
+  return tile_stages<T, DP, kVec>() * (2 * Frags<T>::kTile * Tile<T, DP>::kLd * sizeof(T) + kBiasSpan * sizeof(float));
 }
 
 template <typename T, int DP, bool kVec>
 int launch_forward(const AttnCall& a, void* out, float2* stats, hipStream_t s) {
-  const int64_t blocks = (int64_t)((a.q_len + kAttnRows - 1) / kAttnRows) * a.q_heads * a.batch;
+  const int64_t blocks = query_blocks(a).blocks();
   if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_forward: too many rows");
-  const size_t lds = forward_lds<T, DP>();
+  const size_t lds = forward_lds<T, DP, kVec>();
   const auto kernel = attention_forward_kernel<T, DP, kVec>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, static_cast<T*>(out), stats);
@@ -270,18 +276,18 @@ int64_t mask_words_row(const mdl_attention& a) { return (a.k_len + 63) / 64 + 1;
 
 // Where a prepared call's parts lie.
 struct PrepareLayout {
-  size_t words = 0, first = 0, bias = 0, bytes = 0;
+  size_t words = 0, bounds = 0, bias = 0, bytes = 0;
   explicit PrepareLayout(const mdl_attention& a) {
     size_t at = 0;
     if (a.mask) {
       words = at;
       at = align256(at + (size_t)a.batch * mask_words_row(a) * 8);
-      first = at;
-      at = align256(at + (size_t)a.batch * 4);
+      bounds = at;
+      at = align256(at + (size_t)a.batch * 8);
     }
     if (a.bias_table) {
       bias = at;
-      at = align256(at + (size_t)a.q_heads * a.distances * 4);
+      at = align256(at + (size_t)a.q_heads * (a.distances + 2 * kBiasEdge) * 4);
     }
     bytes = at;
   }
@@ -292,7 +298,7 @@ int attention_check(const mdl_attention* a, const char* what) {
   if (!a) return fail(MDL_ERR_INVALID, w + ": null descriptor");
   if (a->batch < 0 || a->q_len < 0 || a->k_len < a->q_len)
     return fail(MDL_ERR_INVALID, w + ": needs batch >= 0 and 0 <= q_len <= k_len");
-  if (a->batch > 0x7fffffff || a->k_len > 0x3fffffff) return fail(MDL_ERR_UNSUPPORTED, w + ": too many rows");
+  if (a->k_len > 0x3fffffff || (a->batch > 0 && a->q_heads > 0x7fffffff / a->batch)) return fail(MDL_ERR_UNSUPPORTED, w + ": too many rows");
   if (a->q_heads <= 0 || a->kv_heads <= 0 || a->q_heads % a->kv_heads)
     return fail(MDL_ERR_INVALID, w + ": q_heads must be a positive multiple of kv_heads");
   if (a->head_dim <= 0 || a->head_dim > 128) return fail(MDL_ERR_UNSUPPORTED, w + ": head_dim must be 1..128");
@@ -320,7 +326,7 @@ AttnCall attention_call(const mdl_attention& a, const void* prepared) {
   c.v_batch = a.v_batch; c.v_row = a.v_row; c.v_head = a.v_head;
   if (a.mask) {
     c.words = reinterpret_cast<const uint64_t*>(p + lay.words);
-    c.first = reinterpret_cast<const int32_t*>(p + lay.first);
+    c.bounds = reinterpret_cast<const int2*>(p + lay.bounds);
     c.words_row = mask_words_row(a);
   }
   if (a.bias_table) c.bias = reinterpret_cast<const float*>(p + lay.bias);
@@ -371,8 +377,8 @@ int mdl_attention_prepare(const mdl_attention* a, void* prepared, size_t prepare
   c.table = a->bias_table;
   c.starts = a->bucket_starts;
   c.words = reinterpret_cast<uint64_t*>(p + lay.words);
-  c.first = reinterpret_cast<int32_t*>(p + lay.first);
-  c.bias = reinterpret_cast<float*>(p + lay.bias);
+  c.bounds = reinterpret_cast<int2*>(p + lay.bounds);
+  c.bias = a->bias_table ? reinterpret_cast<float*>(p + lay.bias) : nullptr;
   c.words_row = mask_words_row(*a);
   c.batch = (int32_t)a->batch;
   c.k_len = (int32_t)a->k_len;
@@ -381,7 +387,7 @@ int mdl_attention_prepare(const mdl_attention* a, void* prepared, size_t prepare
   c.distances = a->bias_table ? a->distances : 0;
   c.table_f32 = a->table_dtype == MDL_F32;
   c.inv_scale = 1.f / a->scale;
-  const int64_t blocks = (a->mask ? a->batch : 0) + ((int64_t)c.heads * c.distances + 255) / 256;
+  const int64_t blocks = (a->mask ? a->batch : 0) + (c.bias ? ((int64_t)c.heads * (c.distances + 2 * kBiasEdge) + 255) / 256 : 0);
   hipLaunchKernelGGL(attention_prepare_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), c);
   MDL_CHECK_LAUNCH("attention_prepare_kernel");
   return MDL_OK;

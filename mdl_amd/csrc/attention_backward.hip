@@ -23,11 +23,11 @@ namespace mdl {
 
 struct GradCall {
   const void* out;
-  const float2* stats;
+  const float2* stats;  // -m, -log2 of the sum
   const void* grad_out;
   int64_t g_batch, g_row, g_head;
   void *dq, *dk, *dv;
-  float* delta;         // [B, Hq, Lq]
+  float* delta;         // [B, Hq, Lq], negated
   const int32_t* starts;
   int32_t buckets;
   float* bias_partial;  // [Hq, bias_parts, buckets]; NULL: no bias gradient
@@ -46,30 +46,31 @@ template <typename T, int DP, bool kVec>
 __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall a, GradCall g) {
   using F = Frags<T>;
   using Stage = TileStage<T, DP, kVec>;
-  constexpr int TK = F::kTile, LD = Stage::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;
-  constexpr int kBias = kAttnRows + TK;
+  constexpr int TK = F::kTile, LD = Tile<T, DP>::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;
+  constexpr int kStages = tile_stages<T, DP, kVec>();
   extern __shared__ __align__(16) char smem[];
-  T* lds = reinterpret_cast<T*>(smem);
-  float* lds_bias = reinterpret_cast<float*>(lds + 4 * TK * LD);
+  T* lds = reinterpret_cast<T*>(smem);                                       // [stages][K, V][TK][LD]
+  float* lds_bias = reinterpret_cast<float*>(lds + kStages * 2 * TK * LD);  // [stages][kBiasSpan]
 
-  const int blocks_q = (a.q_len + kAttnRows - 1) / kAttnRows;
-  int64_t id = xcd_block(blockIdx.x, gridDim.x);
-  const int qb = blocks_q - 1 - (int)(id % blocks_q);
-  id /= blocks_q;
-  const int head = (int)(id % a.q_heads), b = (int)(id / a.q_heads);
+  int unit, inner;
+  const BlockOrder order = query_blocks(a);
+  if (!order.place(blockIdx.x, &unit, &inner)) return;
+  const int qb = order.per_unit - 1 - inner;  // last rows first: without a window they walk the most tiles
+  const int b = unit / a.q_heads, head = unit - b * a.q_heads;
   const int kv = head / (a.q_heads / a.kv_heads);
   const T* kp = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
-  const float* bias = a.bias ? a.bias + (int64_t)head * a.distances : nullptr;
+  const float* bias = a.bias ? head_bias(a, head) : nullptr;
 
   const int off = a.k_len - a.q_len;
   const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
   const int r0 = qb * kAttnRows;
   const int r_end = r0 + kAttnRows < a.q_len ? r0 + kAttnRows : a.q_len;
   const int row = r0 + 32 * wave + l32, c = row + off;
-  KeyWalk walk(a, b, TK, r0 + off, r_end - 1 + off);
+  const RowMask mask(a, b);
+  const KeyWalk walk(a, mask, TK, r0 + off, r_end - 1 + off);
   const int wc_lo = r0 + 32 * wave + off;
-  const uint32_t q_bits = wc_lo - off < a.q_len ? columns32(a, walk.words, wc_lo) : 0;
+  const uint32_t q_bits = mask.bits32(wc_lo);
   const bool live = (q_bits >> l32) & 1;
 
   typename F::Frag q[kSteps], go[kSteps];
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
                             live, a.dim, q);
   load_own_row<T, DP, kVec>(
       static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head + (int64_t)row * g.g_row, live, a.dim, go);
-  float m = 0.f, ll = INFINITY, delta = 0.f;
+  float m_neg = 0.f, ll_neg = -INFINITY, delta = 0.f;
   {
     typename F::Frag o[kSteps];
     load_own_row<T, DP, kVec>(static_cast<const T*>(g.out) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim,
@@ -89,102 +90,81 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
     delta = sum_halves(delta);
     if (row < a.q_len) {
       const float2 st = g.stats[((int64_t)b * a.q_heads + head) * a.q_len + row];
-      m = st.x;
-      ll = st.y;
+      m_neg = st.x;
+      ll_neg = st.y;
     }
   }
   f32x16 acc[DP / 32], pk[DP / 32];  // sums of dS k and of p k
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = pk[i] = (f32x16)(0.f);
   float rest = 0.f;  // sum of dS: delta less dO . out
-  const f32x16 far_from = (f32x16)((bias ? bias[a.distances - 1] : 0.f) - m), minus_delta = (f32x16)(-delta);
+  const float far_from = (bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f) + m_neg;
 
-  const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
+  const Tile<T, DP> read;
   Stage ks, vs;
-  float bias_next = 0.f;
-  auto fetch = [&](int t, uint64_t bits) {
-    ks.load(kp, a.k_row, t * TK, bits, a.dim);
-    vs.load(vp, a.v_row, t * TK, bits, a.dim);
-    if (bias && threadIdx.x < kBias) {
-      int d = r0 + off - t * TK + kAttnRows - 1 - (int)threadIdx.x;
-      d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
-      bias_next = bias[d];
+  auto fetch = [&](int i, int slot) {
+    const int j0 = walk.tile_at(i) * TK;
+    const uint64_t bits = mask.bits<TK>(j0);
+    T* to = lds + slot * 2 * TK * LD;
+    ks.fetch(to, kp, a.k_row, j0, bits, a.dim);
+    vs.fetch(to + TK * LD, vp, a.v_row, j0, bits, a.dim);
+    if (bias)
+      copy4_to_lds(lds_bias + slot * kBiasSpan + wave * kWave, bias + bias_at(a, r0 + off - j0 - (TK - 1)) + threadIdx.x);
+  };
+  auto settle = [&](int slot) {
+    ks.settle(lds + slot * 2 * TK * LD);
+    vs.settle(lds + slot * 2 * TK * LD + TK * LD);
+  };
+  auto work = [&](int i, int slot) {
+    const T* lk = lds + slot * 2 * TK * LD;
+    const T* lv = lk + TK * LD;
+    const int j0 = walk.tile_at(i) * TK, j1 = j0 + TK - 1;
+    const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
+    if (!seen) return;
+    const uint64_t bits = mask.bits<TK>(j0);
+    const bool far = !bias || wc_lo - j1 >= a.distances - 1;
+    const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
+                       wc_lo + 31 - j0 < a.window;
+#pragma unroll
+    for (int s = 0; s < kSubs; ++s) {
+      f32x16 x, dp = (f32x16)(-delta);
+      if (far) {
+        x = (f32x16)(far_from);
+      } else {
+        const float* from = lds_bias + slot * kBiasSpan + (32 * wave + l32 + TK - 1 - 32 * s - 4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = from[-(8 * (i >> 2) + (i & 3))] + m_neg;
+      }
+      {
+        const NatFrags<T, DP> kn(read, lk, s), vn(read, lv, s);
+        reads_first<T>();
+        x = kn.times(q, x);
+        dp = vn.times(go, dp);
+      }
+      const TrFrags<T, DP> kt(read, lk, s);
+      reads_first<T>();
+      if (!whole) {
+        uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
+        vis >>= 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, ll_neg));
+        dp[i] *= x[i];
+        rest += dp[i];
+      }
+      // p and dS take the element type for the products with k
+      kt.times(dp, acc);
+      kt.times(x, pk);
     }
   };
-  uint64_t bits = 0, bits_next = 0;
-  int t = walk.begin(a, &bits);
-  if (t <= walk.last_tile) fetch(t, bits);
-  int buf = 0;
-  while (t <= walk.last_tile) {
-    T* lk = lds + buf * 2 * TK * LD;
-    T* lv = lk + TK * LD;
-    float* lb = lds_bias + buf * kBias;
-    ks.store(lk);
-    vs.store(lv);
-    if (bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
-    const int t_next = walk.seek(a, t + 1, &bits_next);
-    if (t_next <= walk.last_tile) fetch(t_next, bits_next);
-    __syncthreads();
+  walk_tiles<kStages, 2 * Stage::kPer, Stage::kDirect>(walk.tiles, bias != nullptr, fetch, settle, work);
 
-    const int j0 = t * TK, j1 = j0 + TK - 1;
-    const bool seen = q_bits && j0 <= wc_lo + 31 && (wc_lo - j1 < a.window || j0 < walk.sink_end);
-    if (seen) {
-      const bool far = !bias || wc_lo - j1 >= a.distances - 1;
-      const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
-                         wc_lo + 31 - j0 < a.window;
-#pragma unroll
-      for (int s = 0; s < kSubs; ++s) {
-        f32x16 x, dp;
-        auto products = [&](f32x16 from) {
-          x = F::mma(load_frag(lk + nat + 32 * s * LD), q[0], from);
-          dp = F::mma(load_frag(lv + nat + 32 * s * LD), go[0], minus_delta);
-#pragma unroll
-          for (int d = 1; d < kSteps; ++d) {
-            x = F::mma(load_frag(lk + nat + 32 * s * LD + d * F::kStep), q[d], x);
-            dp = F::mma(load_frag(lv + nat + 32 * s * LD + d * F::kStep), go[d], dp);
-          }
-        };
-        if (far) {
-          products(far_from);
-        } else {
-          const float* from = lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half);
-          f32x16 near;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) near[i] = from[8 * (i >> 2) + (i & 3)] - m;
-          products(near);
-        }
-        if (!whole) {
-          uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
-          vis >>= 4 * half;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, -ll));
-          dp[i] *= x[i];
-          rest += dp[i];
-        }
-        // p and dS take the element type for the products with k
-#pragma unroll
-        for (int p = 0; p < 32 / F::kStep; ++p) {
-          const typename F::Frag pf = F::from_result(x, p), sf = F::from_result(dp, p);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt) {
-            const typename F::Frag kt = F::load_t(lk + tr + (32 * s + F::kStep * p) * LD + 32 * dt, LD);
-            acc[dt] = F::mma(kt, sf, acc[dt]);
-            pk[dt] = F::mma(kt, pf, pk[dt]);
-          }
-        }
-      }
-    }
-    t = t_next;
-    bits = bits_next;
-    buf ^= 1;
-  }
   rest = sum_halves(rest);
   if (row >= a.q_len) return;
-  if (half == 0) g.delta[((int64_t)b * a.q_heads + head) * a.q_len + row] = delta + rest;
+  if (half == 0) g.delta[((int64_t)b * a.q_heads + head) * a.q_len + row] = -(delta + rest);
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -273,6 +253,7 @@ template <typename T, int DP>
 struct KeyTile {
   using F = Frags<T>;
   static constexpr int kSteps = DP / F::kStep;
+  Tile<T, DP> read;
   typename F::Frag k[kSteps], v[kSteps];
   f32x16 dk[DP / 32], dv[DP / 32];
 
@@ -286,19 +267,19 @@ struct KeyTile {
     for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = (f32x16)(0.f);
   }
 
-  // Adds the tile to dk and dv; returns dS.  q, go: the 32 staged rows; rows:
-  // their -m, -log2 sum and -delta, pitch apart; near_bias: the pairs' biases
+  // Adds the tile to dk and dv; returns dS.  q, go: the 32 staged rows; stats,
+  // delta: theirs (-m and -log2 sum; -delta); near_bias: the pairs' biases
   // by row (NULL: all far_bias); vis: the visible rows of the lane's key.
-  __device__ __forceinline__ f32x16 add(const T* q, const T* go, int LD, const float* rows, int pitch, float far_bias,
+  __device__ __forceinline__ f32x16 add(const T* q, const T* go, const float* stats, const float* delta, float far_bias,
                                         const float* near_bias, bool whole, uint32_t vis, float c2) {
-    const int l32 = lane_id() & 31, half = lane_id() >> 5;
-    const int nat = l32 * LD + half * F::kElems, tr = F::t_offset(LD);
-    rows += 4 * half;
+    const int half = lane_id() >> 5;
+    stats += 8 * half;
+    delta += 4 * half;
     f32x16 x, dp;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      x[i] = rows[8 * (i >> 2) + (i & 3)];
-      dp[i] = rows[2 * pitch + 8 * (i >> 2) + (i & 3)];
+      x[i] = stats[2 * (8 * (i >> 2) + (i & 3))];
+      dp[i] = delta[8 * (i >> 2) + (i & 3)];
     }
     if (near_bias) {
 #pragma unroll
@@ -307,34 +288,25 @@ struct KeyTile {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] += far_bias;
     }
-#pragma unroll
-    for (int d = 0; d < kSteps; ++d) {
-      x = F::mma(load_frag(q + nat + d * F::kStep), k[d], x);
-      dp = F::mma(load_frag(go + nat + d * F::kStep), v[d], dp);
+    {
+      const NatFrags<T, DP> qn(read, q, 0), gn(read, go, 0);
+      reads_first<T>();
+      x = qn.times(k, x);
+      dp = gn.times(v, dp);
     }
+    const TrFrags<T, DP> gt(read, go, 0), qt(read, q, 0);
+    reads_first<T>();
     if (!whole) {
       vis >>= 4 * half;
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], c2, rows[pitch + 8 * (i >> 2) + (i & 3)]));
-#pragma unroll
-    for (int p = 0; p < 32 / F::kStep; ++p) {
-      const typename F::Frag pf = F::from_result(x, p);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-        dv[dt] = F::mma(F::load_t(go + tr + F::kStep * p * LD + 32 * dt, LD), pf, dv[dt]);
-    }
+    for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], c2, stats[2 * (8 * (i >> 2) + (i & 3)) + 1]));
+    gt.times(x, dv);
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] *= dp[i];
-#pragma unroll
-    for (int p = 0; p < 32 / F::kStep; ++p) {
-      const typename F::Frag sf = F::from_result(x, p);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-        dk[dt] = F::mma(F::load_t(q + tr + F::kStep * p * LD + 32 * dt, LD), sf, dk[dt]);
-    }
+    qt.times(x, dk);
     return x;
   }
 };
@@ -401,105 +373,81 @@ template <typename T, int DP, bool kVec>
 __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCall a, GradCall g) {
   using F = Frags<T>;
   using Stage = TileStage<T, DP, kVec>;
-  constexpr int TQ = F::kTile, LD = Stage::kLd, kSubs = TQ / 32;
-  constexpr int kBias = kAttnRows + TQ;
+  constexpr int TQ = F::kTile, LD = Tile<T, DP>::kLd, kSubs = TQ / 32;
+  constexpr int kStages = 2;  // a third would leave LDS for one block beside the bias sums
   extern __shared__ __align__(16) char smem[];
-  T* lds = reinterpret_cast<T*>(smem);                           // [2][Q, dO][TQ][LD]
-  float* lds_row = reinterpret_cast<float*>(lds + 4 * TQ * LD);  // [2][-m, -log2 sum, -delta][TQ]
-  float* lds_bias = lds_row + 6 * TQ;                            // [2][kBias]
+  T* lds = reinterpret_cast<T*>(smem);                                      // [stages][Q, dO][TQ][LD]
+  float* lds_row = reinterpret_cast<float*>(lds + kStages * 2 * TQ * LD);  // [stages][(-m, -log2 sum)[TQ], -delta[TQ], ..]
+  float* lds_bias = lds_row + kStages * kAttnThreads;                      // [stages][kBiasSpan]
 
   const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
   const int key_blocks = (a.k_len + kAttnRows - 1) / kAttnRows;
-  int64_t id = xcd_block(blockIdx.x, gridDim.x);
-  const int kb = (int)(id % key_blocks);  // first keys first: without a window they walk the most tiles
-  id /= key_blocks;
-  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
-  const uint64_t* words = a.words ? a.words + (int64_t)b * a.words_row : nullptr;
+  int unit, kb;  // first keys first: without a window they walk the most tiles
+  if (!key_unit_blocks(a, key_blocks).place(blockIdx.x, &unit, &kb)) return;
+  const int b = unit / a.kv_heads, kv = unit - b * a.kv_heads;
+  const RowMask mask(a, b);
 
   const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
-  const int k0 = kb * kAttnRows, k_end = a.k_len;
+  const int k0 = kb * kAttnRows;
   const int jw = k0 + 32 * wave, j = jw + l32;
-  const uint32_t k_bits = columns32(a, words, jw);
+  const uint32_t k_bits = mask.bits32(jw);
   const bool live = (k_bits >> l32) & 1;
 
   KeyTile<T, DP> tile;
   tile.template open<kVec>(a, b, kv, j, live);
   const bool want_bias = g.bias_partial != nullptr;
   BlockBias sums;
-  if (want_bias) sums.open(a, lds_bias + 2 * kBias, off - k0);
+  if (want_bias) sums.open(a, lds_bias + kStages * kBiasSpan, off - k0);
   const int64_t part = (int64_t)b * key_blocks + kb;
 
-  // query rows with a pair here
-  int r_lo = k0 - off, r_hi = (k_end < k0 + kAttnRows ? k_end : k0 + kAttnRows) - 1 + a.window - 1 - off;
-  if (r_lo < 0) r_lo = 0;
-  if (r_hi > a.q_len - 1) r_hi = a.q_len - 1;
-  const int t_first = r_lo / TQ, t_last = r_lo <= r_hi ? r_hi / TQ : -1;
+  // columns of the queries with a pair here, as tiles of query rows
+  int c_lo = k0 > mask.first ? k0 : mask.first, c_hi = k0 + kAttnRows - 1 + a.window - 1;
+  if (c_hi > mask.last) c_hi = mask.last;
+  if (c_lo < off) c_lo = off;
+  const int t_first = (c_lo - off) / TQ;
+  const int per_head = c_lo <= c_hi && k0 <= mask.last ? (c_hi - off) / TQ - t_first + 1 : 0;
 
   Stage qs, gs;
-  float2 stat_next = make_float2(0.f, INFINITY);
-  float delta_next = 0.f, bias_next = 0.f;
-  auto row_bits = [&](int t) {
-    const uint32_t lo = columns32(a, words, t * TQ + off);
-    if (TQ == 32) return (uint64_t)lo;
-    return lo | (uint64_t)columns32(a, words, t * TQ + off + 32) << 32;
-  };
-  // (head of the group, tile) from (hs, t) on with an unmasked query
-  auto seek = [&](int& hs, int& t, uint64_t& bits) {
-    for (; hs < share; ++hs, t = t_first)
-      for (; t <= t_last; ++t) {
-        bits = row_bits(t);
-        if (bits) return;
-      }
-  };
-  auto fetch = [&](int hs, int t, uint64_t bits) {
-    const int head = kv * share + hs;
-    qs.load(static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head, a.q_row, t * TQ, bits, a.dim);
-    gs.load(static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head, g.g_row, t * TQ, bits, a.dim);
-    if (threadIdx.x < TQ) {
-      const int r = t * TQ + (int)threadIdx.x;
-      const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + r;
-      stat_next = r < a.q_len ? g.stats[at] : make_float2(0.f, INFINITY);
-      delta_next = r < a.q_len ? g.delta[at] : 0.f;
+  int fetch_head = 0, fetch_tile = 0;  // the next pair to fetch: head of the group, tile of the walk
+  auto fetch = [&](int, int slot) {
+    const int head = kv * share + fetch_head, row0 = (t_first + fetch_tile) * TQ;
+    if (++fetch_tile == per_head) {
+      fetch_tile = 0;
+      ++fetch_head;
     }
-    if (a.bias && threadIdx.x < kBias) {
-      // lds_bias[i]: the distance of query q' and key k' with q' - k' = i - (rows - 1)
-      int d = t * TQ + off - k0 - (kAttnRows - 1) + (int)threadIdx.x;
-      d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
-      bias_next = a.bias[(int64_t)head * a.distances + d];
+    const uint64_t bits = mask.bits<TQ>(row0 + off);
+    T* to = lds + slot * 2 * TQ * LD;
+    qs.fetch(to, static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head, a.q_row, row0, bits, a.dim);
+    gs.fetch(to + TQ * LD, static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head, g.g_row, row0, bits,
+             a.dim);
+    // one float a thread: the rows' statistics, then their delta (rows past the last one take its)
+    {
+      const int n = threadIdx.x, most = a.q_len - 1;
+      const int r = n < 2 * TQ ? row0 + (n >> 1) : row0 + ((n - 2 * TQ) & (TQ - 1));
+      const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + (r < most ? r : most);
+      const float* from = n < 2 * TQ ? reinterpret_cast<const float*>(g.stats + at) + (n & 1) : g.delta + at;
+      copy4_to_lds(lds_row + slot * kAttnThreads + wave * kWave, from);
     }
+    // lds_bias[i]: distance i + that of the tile's first query and the block's last key
+    if (a.bias)
+      copy4_to_lds(lds_bias + slot * kBiasSpan + wave * kWave,
+                   head_bias(a, head) + bias_at(a, row0 + off - k0 - (kAttnRows - 1)) + threadIdx.x);
   };
-
-  int hs = 0, t = t_first;
-  uint64_t bits = 0, bits_next = 0;
-  if (t_last < 0) hs = share;
-  seek(hs, t, bits);
-  if (hs < share) fetch(hs, t, bits);
-  else if (want_bias)
-    for (int i = 0; i < share; ++i) sums.leave(a, g, kv * share + i, part);
-  int buf = 0;
-  while (hs < share) {
-    T* lq = lds + buf * 2 * TQ * LD;
-    T* lg = lq + TQ * LD;
-    float* lr = lds_row + buf * 3 * TQ;
-    float* lb = lds_bias + buf * kBias;
-    qs.store(lq);
-    gs.store(lg);
-    if (threadIdx.x < TQ) {
-      lr[threadIdx.x] = -stat_next.x;
-      lr[TQ + threadIdx.x] = -stat_next.y;
-      lr[2 * TQ + threadIdx.x] = -delta_next;
-    }
-    if (a.bias && threadIdx.x < kBias) lb[threadIdx.x] = bias_next;
-    int hs_next = hs, t_next = t + 1;
-    seek(hs_next, t_next, bits_next);
-    if (hs_next < share) fetch(hs_next, t_next, bits_next);
-    __syncthreads();
-
-    const int c0 = t * TQ + off, c1 = c0 + TQ - 1;
+  auto settle = [&](int slot) {
+    qs.settle(lds + slot * 2 * TQ * LD);
+    gs.settle(lds + slot * 2 * TQ * LD + TQ * LD);
+  };
+  int hs = 0, t = 0;
+  float far_bias = a.bias ? load_uniform(head_bias(a, kv * share) + kBiasEdge + a.distances - 1) : 0.f;
+  auto work = [&](int, int slot) {
+    const T* lq = lds + slot * 2 * TQ * LD;
+    const T* lg = lq + TQ * LD;
+    const float* lr = lds_row + slot * kAttnThreads;
+    const float* lb = lds_bias + slot * kBiasSpan;
+    const int c0 = (t_first + t) * TQ + off, c1 = c0 + TQ - 1;
     const bool seen = k_bits && c1 >= jw && c0 - (jw + 31) < a.window;
     if (seen) {
-      // of the tile's largest distance: the far bias if any of its products is far
-      const float far_bias = a.bias ? lb[kAttnRows - 32 - 32 * wave + TQ - 32] : 0.f;
+      const uint64_t bits = mask.bits<TQ>(c0);
       const bool whole = k_bits == ~0u && (TQ == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && c0 >= jw + 31 &&
                          c1 - jw < a.window;
 #pragma unroll
@@ -510,21 +458,26 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
         if (!whole)
           vis = live ? ~low_bits(j - col) & low_bits(j + a.window - col) & (uint32_t)(bits >> (32 * s)) : 0u;
         const f32x16 ds =
-            tile.add(lq + 32 * s * LD, lg + 32 * s * LD, LD, lr + 32 * s, TQ, far_bias,
+            tile.add(lq + 32 * s * LD, lg + 32 * s * LD, lr + 64 * s, lr + 2 * TQ + 32 * s, far_bias,
                      far ? nullptr : lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half), whole, vis, a.c2);
         if (want_bias) sums.add(ds, corner, far);
       }
     }
-    if (want_bias && hs_next != hs) sums.leave(a, g, kv * share + hs, part);
-    hs = hs_next;
-    t = t_next;
-    bits = bits_next;
-    buf ^= 1;
-  }
+    if (++t == per_head) {
+      if (want_bias) sums.leave(a, g, kv * share + hs, part);
+      t = 0;
+      ++hs;
+      if (a.bias && hs < share)
+        far_bias = load_uniform(head_bias(a, kv * share + hs) + kBiasEdge + a.distances - 1);
+    }
+  };
+  walk_tiles<kStages, 2 * Stage::kPer + 1, Stage::kDirect>(per_head * share, a.bias != nullptr, fetch, settle, work);
+  if (want_bias && per_head == 0)
+    for (int i = 0; i < share; ++i) sums.leave(a, g, kv * share + i, part);
 
   if (j >= a.k_len) return;
   if (g.far_partial) {
-    const int first = a.words ? a.first[b] : 0;
+    const int first = mask.first;
     if (j >= first && j - first < a.sinks) {
 #pragma unroll 2
       for (int n = 0; n < g.far_chunks; ++n) {
@@ -561,29 +514,27 @@ __host__ __device__ constexpr int far_waves() { return sizeof(T) == 4 && DP == 1
 template <typename T, int DP, bool kVec>
 __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCall a, GradCall g) {
   using F = Frags<T>;
-  constexpr int LD = TileStage<T, DP, kVec>::kLd, kPieces = DP / F::kElems, kPer = 32 * kPieces / kWave;
+  constexpr int LD = Tile<T, DP>::kLd, kPieces = DP / F::kElems, kPer = 32 * kPieces / kWave;
   constexpr int kBias = 64, kWalk = far_waves<T, DP>();
   extern __shared__ __align__(16) char smem[];
   const int wave = wave_id(), l32 = lane_id() & 31, half = lane_id() >> 5;
   T* lq = reinterpret_cast<T*>(smem) + wave * 64 * LD;  // of the wave: [Q, dO][32][LD]
   T* lg = lq + 32 * LD;
   float* lr = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + kWalk * 64 * LD) + wave * (96 + kBias);
-  float* lb = lr + 96;
+  float* lb = lr + 96;  // lr: (-m, -log2 sum)[32], -delta[32]
   float* joined = reinterpret_cast<float*>(smem);  // [dk, dv][32][dim], after the walk
 
   const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
   const int key_blocks = (a.sinks + 31) / 32;
-  int64_t id = xcd_block(blockIdx.x, gridDim.x);
-  const int kb = (int)(id % key_blocks);
-  id /= key_blocks;
-  const int chunk = (int)(id % g.far_chunks);
-  id /= g.far_chunks;
-  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
-  const uint64_t* words = a.words ? a.words + (int64_t)b * a.words_row : nullptr;
-  const int first = a.words ? a.first[b] : 0;
+  int unit, inner;
+  if (!key_unit_blocks(a, key_blocks * g.far_chunks).place(blockIdx.x, &unit, &inner)) return;
+  const int kb = inner % key_blocks, chunk = inner / key_blocks;
+  const int b = unit / a.kv_heads, kv = unit - b * a.kv_heads;
+  const RowMask mask(a, b);
+  const int first = mask.first;
   const int k_end = first + a.sinks < a.k_len ? first + a.sinks : a.k_len;
   const int k0 = first + 32 * kb, j = k0 + l32;
-  const uint32_t k_bits = columns32(a, words, k0) & low_bits(k_end - k0);
+  const uint32_t k_bits = mask.bits32(k0) & low_bits(k_end - k0);
   const bool live = (k_bits >> l32) & 1;
 
   KeyTile<T, DP> tile;
@@ -597,12 +548,12 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
   const int r_first = chunk * kFarRows, r_last = r_first + kFarRows < a.q_len ? r_first + kFarRows : a.q_len;
   for (int hs = 0; hs < share; ++hs) {
     const int head = kv * share + hs;
-    const float far_bias = a.bias ? a.bias[(int64_t)head * a.distances + a.distances - 1] : 0.f;
+    const float far_bias = a.bias ? load_uniform(head_bias(a, head) + kBiasEdge + a.distances - 1) : 0.f;
     const T* qp = static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head;
     const T* gp = static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head;
     for (int r0 = r_first + 32 * wave; wave < kWalk && r0 < r_last; r0 += 32 * kWalk) {
       const int col = r0 + off;
-      const uint32_t bits = columns32(a, words, col);
+      const uint32_t bits = mask.bits32(col);
       if (!k_bits || !bits || col + 31 < k0 + a.window) continue;
       typename F::Frag qr[kPer], gr[kPer];
 #pragma unroll
@@ -614,7 +565,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
           gr[i] = load_row<T, kVec>(gp + (int64_t)(r0 + row) * g.g_row, d, a.dim);
         }
       }
-      float2 st = make_float2(0.f, INFINITY);
+      float2 st = make_float2(0.f, -INFINITY);
       float delta = 0.f;
       if (r0 + l32 < a.q_len) {
         const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + r0 + l32;
@@ -626,28 +577,26 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
       float near = 0.f;
       if (!far) {
         // lb[i]: distance corner - 31 + i
-        int d = corner - 31 + lane_id();
-        d = d < 0 ? 0 : (d < a.distances ? d : a.distances - 1);
-        near = a.bias[(int64_t)head * a.distances + d];
+        near = head_bias(a, head)[bias_at(a, corner - 31) + lane_id()];
       }
       wave_sync();
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int at = i * kWave + lane_id();
-        *reinterpret_cast<typename F::Frag*>(lq + at / kPieces * LD + at % kPieces * F::kElems) = qr[i];
-        *reinterpret_cast<typename F::Frag*>(lg + at / kPieces * LD + at % kPieces * F::kElems) = gr[i];
+        *reinterpret_cast<typename F::Frag*>(lq + Tile<T, DP>::place(at / kPieces, at % kPieces)) = qr[i];
+        *reinterpret_cast<typename F::Frag*>(lg + Tile<T, DP>::place(at / kPieces, at % kPieces)) = gr[i];
       }
       if (half == 0) {
-        lr[l32] = -st.x;
-        lr[32 + l32] = -st.y;
-        lr[64 + l32] = -delta;
+        lr[2 * l32] = st.x;
+        lr[2 * l32 + 1] = st.y;
+        lr[64 + l32] = delta;
       }
       if (!far) lb[lane_id()] = near;
       wave_sync();
       const bool whole = k_bits == ~0u && bits == ~0u && corner - 31 >= a.window;
       const uint32_t vis = live ? ~low_bits(j + a.window - col) & bits : 0u;
       const f32x16 ds =
-          tile.add(lq, lg, LD, lr, 32, far_bias, far ? nullptr : lb + 31 - l32 + 4 * half, whole, vis, a.c2);
+          tile.add(lq, lg, lr, lr + 64, far_bias, far ? nullptr : lb + 31 - l32 + 4 * half, whole, vis, a.c2);
       if (want_bias) sums.add(ds, corner, far);
     }
     if (want_bias) sums.leave(a, g, head, part);
@@ -705,9 +654,10 @@ struct BackwardLayout {
 template <typename T, int DP, bool kVec>
 int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
   using F = Frags<T>;
-  const size_t tiles = (size_t)4 * F::kTile * TileStage<T, DP, true>::kLd * sizeof(T) + 2 * (kAttnRows + F::kTile) * sizeof(float);
+  constexpr int kStages = tile_stages<T, DP, kVec>();
+  const size_t tiles = kStages * (2 * F::kTile * Tile<T, DP>::kLd * sizeof(T) + kBiasSpan * sizeof(float));
   {
-    const int64_t blocks = (int64_t)((a.q_len + kAttnRows - 1) / kAttnRows) * a.q_heads * a.batch;
+    const int64_t blocks = query_blocks(a).blocks();
     const auto kernel = attention_grad_q_kernel<T, DP, kVec>;
     if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
     if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), tiles)) return rc;
@@ -717,9 +667,9 @@ int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
   const size_t bias_lds =
       g.bias_partial ? (size_t)4 * (32 * kSkew + ((a.distances + 2 * kSpare + 3) & ~3)) * sizeof(float) : 0;
   if (g.far_partial) {
-    const int64_t blocks = (int64_t)((a.sinks + 31) / 32) * g.far_chunks * a.kv_heads * a.batch;
+    const int64_t blocks = key_unit_blocks(a, (a.sinks + 31) / 32 * g.far_chunks).blocks();
     const size_t walk =
-        far_waves<T, DP>() * ((size_t)64 * TileStage<T, DP, true>::kLd * sizeof(T) + (96 + 64) * sizeof(float)) + bias_lds;
+        far_waves<T, DP>() * ((size_t)64 * Tile<T, DP>::kLd * sizeof(T) + (96 + 64) * sizeof(float)) + bias_lds;
     const size_t join = (size_t)2 * DP * 32 * sizeof(float);
     const size_t lds = walk > join ? walk : join;
     const auto kernel = attention_grad_far_kernel<T, DP, kVec>;
@@ -728,8 +678,8 @@ int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
     MDL_CHECK_LAUNCH("attention_grad_far_kernel");
   }
-  const size_t lds = tiles + (size_t)6 * F::kTile * sizeof(float) + bias_lds;
-  const int64_t blocks = (int64_t)((a.k_len + kAttnRows - 1) / kAttnRows) * a.kv_heads * a.batch;
+  const size_t lds = 2 * (2 * F::kTile * Tile<T, DP>::kLd * sizeof(T) + (kBiasSpan + kAttnThreads) * sizeof(float)) + bias_lds;
+  const int64_t blocks = key_unit_blocks(a, (a.k_len + kAttnRows - 1) / kAttnRows).blocks();
   const auto kernel = attention_grad_kv_kernel<T, DP, kVec>;
   if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;

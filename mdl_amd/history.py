@@ -222,9 +222,9 @@ def _attention_forward_fake(q, k, v, mask, bias_table, bucket_starts, distances,
             return (n + 255) // 256 * 256
 
         if mask is not None:
-            words += part(k.size(0) * ((k.size(1) + 63) // 64 + 1) * 8) + part(k.size(0) * 4)
+            words += part(k.size(0) * ((k.size(1) + 63) // 64 + 1) * 8) + part(k.size(0) * 8)
         if bias_table is not None:
-            words += part(q.size(2) * distances * 4)
+            words += part(q.size(2) * (distances + 512) * 4)
     return (q.new_empty(q.shape), q.new_empty(_stats_shape(q, need_backward), dtype=torch.float32),
             q.new_empty(words, dtype=torch.uint8))
 
