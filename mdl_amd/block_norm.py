@@ -20,6 +20,8 @@ from torch import Tensor
 from . import library  # noqa: F401  (loads libmdl_torch.so and its schemas)
 from .library import _cpu_kernel, _fake_kernel
 
+_NORM = torch.ops.mdl_hip.gated_residual_norm.default  # looked up once
+
 
 def _check(x, block_out, post_weight, next_weight, gate, residual_scale, eps) -> None:
     if x.ndim < 1 or x.size(-1) < 1:
@@ -139,5 +141,4 @@ def gated_residual_norm(
     most 8192 (bf16) or 4096 (fp32) elements.
     """
 
-    return torch.ops.mdl_hip.gated_residual_norm(x, block_out, post_weight, next_weight, gate, residual_scale,
-                                                 float(eps))
+    return _NORM(x, block_out, post_weight, next_weight, gate, residual_scale, float(eps))

@@ -13,10 +13,14 @@
 
 namespace mdl {
 
-constexpr int kStepThreads = 256;
-constexpr int kStepUnroll = 4;     // rows in flight per lane group
-constexpr int kStepBlocks = 1024;  // blocks wanted before a row's walk is no longer cut
+constexpr int kJoinThreads = 512;
+constexpr int kStepBlocks = 512;   // blocks wanted before a row's walk is no longer cut
 constexpr int kStepMinRows = 512;  // cached rows of a part at least
+
+// Rows of a lane group's iteration: twice as many are in flight (the next
+// iteration's are read while this one's are worked on).
+template <int G>
+constexpr int step_unroll() { return G == 8 ? 2 : 4; }
 
 struct StepCall {
   const void *q, *k, *v;
@@ -26,8 +30,9 @@ struct StepCall {
   const int32_t* starts;
   float* part;  // [B * Hq, parts, 2 + dim]: maximum, sum, sums of values; NULL with one part
   int64_t q_batch, q_head, k_batch, k_head, v_batch, v_head;
-  int64_t ck_batch, ck_slot, ck_head, cv_batch, cv_slot, cv_head;
-  int64_t window, sinks, ring;  // window <= ring
+  int64_t ck_batch, ck_head, cv_batch, cv_head, row_k, row_v;  // row_k, row_v: a prompt's row strides
+  uint32_t ck_slot, cv_slot;
+  int32_t window, sinks, capacity;  // window <= capacity - sinks
   int32_t batch, q_heads, kv_heads, dim, parts, buckets, distances, table_f32;
   float c2;  // scale * log2(e)
 };
@@ -35,33 +40,59 @@ struct StepCall {
 // The cached rows a token at position n sees, in order: the first tokens,
 // then those of the window; the last one is the token itself.
 struct StepRows {
-  int64_t sinks, from, base, ring, at_sinks, count;
+  int sinks, count, shift, capacity, ring, first_distance;
   __device__ __forceinline__ StepRows(const StepCall& a, int64_t n) {
-    sinks = a.sinks < n + 1 ? a.sinks : n + 1;
-    from = n - a.window + 1;
+    capacity = a.capacity;
+    ring = a.capacity - a.sinks;
+    sinks = a.sinks < n + 1 ? a.sinks : (int)(n + 1);
+    int64_t from = n - a.window + 1;
     if (from < a.sinks) from = a.sinks;
-    ring = a.ring;
-    at_sinks = a.sinks;
-    base = from <= n ? (from - a.sinks) % ring : 0;
-    count = sinks + (from <= n ? n - from + 1 : 0);
+    const int in_window = from <= n ? (int)(n - from + 1) : 0;
+    count = sinks + in_window;
+    // slot of the window's first row, less its index
+    int64_t base = from <= n ? from - a.sinks : 0;
+    if (base >= ring) base %= ring;
+    shift = (int)base + a.sinks - sinks;
+    first_distance = n < INT32_MAX ? (int)n : INT32_MAX;
   }
-  __device__ __forceinline__ int64_t position(int64_t i) const { return i < sinks ? i : from + (i - sinks); }
-  __device__ __forceinline__ int64_t slot(int64_t i) const {
-    if (i < sinks) return i;
-    int64_t x = base + (i - sinks);  // the window is no longer than the ring: one turn at most
-    if (x >= ring) x -= ring;
-    return at_sinks + x;
+  __device__ __forceinline__ int slot(int i) const {
+    int t = i + (i < sinks ? 0 : shift);
+    if (t >= capacity) t -= ring;  // the window is no longer than the ring: one turn at most
+    return t;
   }
+  __device__ __forceinline__ int distance(int i) const { return (i < sinks ? first_distance : count - 1) - i; }
   // rows of one part, whole parts of at least kStepMinRows
-  __device__ __forceinline__ int64_t per_part(int parts) const {
-    const int64_t per = (count + parts - 1) / parts;
+  __device__ __forceinline__ int per_part(int parts) const {
+    const int per = (count + parts - 1) / parts;
     return per > kStepMinRows ? per : kStepMinRows;
   }
 };
 
+// row + slot * stride (elements); the product has 64 bits, its factors 32.
+template <typename T>
+__device__ __forceinline__ T* row_at(T* base, int slot, uint32_t stride) {
+  return base + (uint64_t)(uint32_t)slot * stride;
+}
+
 template <typename T>
 __device__ __forceinline__ float element(const typename Frags<T>::Frag& f, int i) {
   return (float)f[i];
+}
+
+// Sum over the lane's elements of two rows, in fp32 (bf16 pairs are multiplied
+// and added to it by one instruction).
+__device__ __forceinline__ float dot(const bf16x8& a, const bf16x8& b) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    t = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a[2 * i], a[2 * i + 1]}, bf16x2{b[2 * i], b[2 * i + 1]}, t, false);
+  return t;
+}
+__device__ __forceinline__ float dot(const f32x4& a, const f32x4& b) {
+  float t = a[0] * b[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) t = __builtin_fmaf(a[i], b[i], t);
+  return t;
 }
 
 // One head group's running softmax over its lanes' values.
@@ -107,39 +138,86 @@ __device__ __forceinline__ void store_piece(T* row, int d, int D, const float* v
     }
 }
 
-template <typename T, int L, int G, bool kVec>
-__global__ __launch_bounds__(kStepThreads) void attention_step_kernel(StepCall a, T* out) {
+// Waves of a block: four, so that several blocks share a CU; eight for calls
+// of at most a block per CU, which end with their one walk (one user's token
+// over 260 rows, 4 heads of 64: 8.7 us with four, 7.0 with eight).
+constexpr int kFewBlocks = 256;
+
+template <typename T, int L, int G, bool kVec, int kWaves>
+__global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall a, T* out) {
   using F = Frags<T>;
-  constexpr int E = F::kElems, kGroups = kWave / L, kWaves = kStepThreads / kWave;
-  constexpr int kPass = kGroups * kStepUnroll;  // rows of a wave's iteration
+  constexpr int E = F::kElems, kGroups = kWave / L, kStepThreads = kWaves * kWave;
+  constexpr int U = step_unroll<G>(), kPass = kGroups * U;  // rows of a wave's iteration
   extern __shared__ __align__(16) char smem[];
   float* lds_table = reinterpret_cast<float*>(smem);           // [buckets][G] bias in powers of two
   uint16_t* lds_bucket = reinterpret_cast<uint16_t*>(lds_table + a.buckets * G);  // [distances]
   __shared__ float lds_join[kWaves][L][G][E + 2];
 
   const int share = a.q_heads / a.kv_heads, groups = (share + G - 1) / G;
-  int64_t id = blockIdx.x;
+  unsigned id = blockIdx.x;
   const int part = (int)(id % a.parts);
   id /= a.parts;
   const int hg = (int)(id % groups);
   id /= groups;
-  const int kv = (int)(id % a.kv_heads), b = (int)(id / a.kv_heads);
+  const int b = (int)(id / a.kv_heads), kv = (int)id - b * a.kv_heads;
   const int head0 = kv * share + hg * G, heads = share - hg * G < G ? share - hg * G : G;
-  const int wave = threadIdx.x / kWave, sub = lane_id() % L, group = lane_id() / L;
+  const int wave = wave_id(), sub = lane_id() % L, group = lane_id() / L;
   const int d = sub * E;
   T* out_row = out + ((int64_t)b * a.q_heads + head0) * a.dim;
 
-  const int64_t n = a.positions[b];
+  const int64_t n = load_uniform(a.positions + b);
   if (n < 0) {  // no such position: nothing stored, zeros answered
     if (part == 0)
       for (int i = threadIdx.x; i < heads * a.dim; i += kStepThreads) out_row[i] = T(0);
     return;
   }
   const StepRows rows(a, n);
-  const int64_t per = rows.per_part(a.parts);
-  const int64_t lo = part * per, hi = lo + per < rows.count ? lo + per : rows.count;
+  const int per = rows.per_part(a.parts);
+  const int lo = part * per, hi = lo + per < rows.count ? lo + per : rows.count;
   if (lo >= hi) return;
 
+  const T* new_k = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
+  const T* new_v = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
+  T* cache_k = static_cast<T*>(a.cache_k) + b * a.ck_batch + kv * a.ck_head;
+  T* cache_v = static_cast<T*>(a.cache_v) + b * a.cv_batch + kv * a.cv_head;
+
+  typename F::Frag q[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    q[g] = {};
+    if (g < heads)
+      q[g] = load_row<T, kVec>(static_cast<const T*>(a.q) + b * a.q_batch + (int64_t)(head0 + g) * a.q_head, d, a.dim);
+  }
+
+  const int last = rows.count - 1;
+  struct Rows {
+    typename F::Frag k[U], v[U];
+  };
+  auto load = [&](Rows& r, int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kGroups + group;
+      r.k[u] = {};
+      r.v[u] = {};
+      if (i < last && i < hi) {
+        const int slot = rows.slot(i);
+        r.k[u] = load_row<T, kVec>(row_at(cache_k, slot, a.ck_slot), d, a.dim);
+        r.v[u] = load_row<T, kVec>(row_at(cache_v, slot, a.cv_slot), d, a.dim);
+      }
+    }
+    if (last < hi && i0 <= last && last < i0 + kPass) {  // the token's own row
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * kGroups + group == last) {
+          r.k[u] = load_row<T, kVec>(new_k, d, a.dim);
+          r.v[u] = load_row<T, kVec>(new_v, d, a.dim);
+        }
+    }
+  };
+  const int first_row = lo + wave * kPass, stride = kWaves * kPass;
+  Rows even, odd;
+  load(even, first_row);
+  // the bias is staged while the first rows are on their way
   if (a.table) {
     for (int i = threadIdx.x; i < a.buckets * G; i += kStepThreads) {
       const int g = i % G;
@@ -163,73 +241,59 @@ __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(StepCall a
     __syncthreads();
   }
 
-  const T* new_k = static_cast<const T*>(a.k) + b * a.k_batch + kv * a.k_head;
-  const T* new_v = static_cast<const T*>(a.v) + b * a.v_batch + kv * a.v_head;
-  T* cache_k = static_cast<T*>(a.cache_k) + b * a.ck_batch + kv * a.ck_head;
-  T* cache_v = static_cast<T*>(a.cache_v) + b * a.cv_batch + kv * a.cv_head;
-
-  float q[G][E];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    typename F::Frag f = {};
-    if (g < heads)
-      f = load_row<T, kVec>(static_cast<const T*>(a.q) + b * a.q_batch + (int64_t)(head0 + g) * a.q_head, d, a.dim);
-#pragma unroll
-    for (int e = 0; e < E; ++e) q[g][e] = element<T>(f, e) * a.c2;
-  }
 
   StepState<G, E> st;
-  const int64_t last = rows.count - 1;
-  for (int64_t i0 = lo + wave * kPass; i0 < hi; i0 += kWaves * kPass) {
-    typename F::Frag kf[kStepUnroll], vf[kStepUnroll];
+  auto work = [&](const Rows& r, int i0) {
+    float s[U][G];
+    // distances of the iteration all in the last bucket (the first tokens' are the largest of all)
+    const bool far = a.table && rows.distance(i0 + kPass - 1) >= a.distances - 1;
 #pragma unroll
-    for (int u = 0; u < kStepUnroll; ++u) {
-      const int64_t i = i0 + u * kGroups + group;
-      kf[u] = {};
-      vf[u] = {};
-      if (i < hi) {
-        const int64_t slot = rows.slot(i);
-        kf[u] = load_row<T, kVec>(i == last ? new_k : cache_k + slot * a.ck_slot, d, a.dim);
-        vf[u] = load_row<T, kVec>(i == last ? new_v : cache_v + slot * a.cv_slot, d, a.dim);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kGroups + group;
+#pragma unroll
+      for (int g = 0; g < G; ++g) s[u][g] = group_sum<L>(dot(q[g], r.k[u]));
+      if (a.table) {
+        const float* bias = lds_table + (a.buckets - 1) * G;
+        if (!far) {
+          const int x = rows.distance(i < hi ? i : hi - 1);
+          if (x < a.distances) bias = lds_table + lds_bucket[x] * G;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) s[u][g] = __builtin_fmaf(s[u][g], a.c2, bias[g]);
+      } else {
+#pragma unroll
+        for (int g = 0; g < G; ++g) s[u][g] *= a.c2;
       }
-    }
-    float s[kStepUnroll][G];
+      if (i0 + kPass > hi) {
 #pragma unroll
-    for (int u = 0; u < kStepUnroll; ++u) {
-      const int64_t i = i0 + u * kGroups + group;
-      const float* bias = nullptr;
-      if (a.table && i < hi) {
-        const int64_t x = n - rows.position(i);
-        bias = lds_table + (x < a.distances ? lds_bucket[x] : a.buckets - 1) * G;
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float t = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) t = __builtin_fmaf(q[g][e], element<T>(kf[u], e), t);
-        t = group_sum<L>(t);
-        if (bias) t += bias[g];
-        s[u][g] = i < hi ? t : -INFINITY;
+        for (int g = 0; g < G; ++g) s[u][g] = i < hi ? s[u][g] : -INFINITY;
       }
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float top = s[0][g];
 #pragma unroll
-      for (int u = 1; u < kStepUnroll; ++u) top = fmaxf(top, s[u][g]);
+      for (int u = 1; u < U; ++u) top = fmaxf(top, s[u][g]);
       if (__any(top > st.m[g] + 8.f)) st.raise(g, fmaxf(st.m[g], top));
 #pragma unroll
-      for (int u = 0; u < kStepUnroll; ++u) {
+      for (int u = 0; u < U; ++u) {
         const float p = exp2_fast(s[u][g] - st.m[g]);
         st.l[g] += p;
 #pragma unroll
-        for (int e = 0; e < E; ++e) st.acc[g][e] = __builtin_fmaf(p, element<T>(vf[u], e), st.acc[g][e]);
+        for (int e = 0; e < E; ++e) st.acc[g][e] = __builtin_fmaf(p, element<T>(r.v[u], e), st.acc[g][e]);
       }
     }
+  };
+  for (int i0 = first_row; i0 < hi; i0 += 2 * stride) {
+    load(odd, i0 + stride);
+    work(even, i0);
+    if (i0 + stride >= hi) break;
+    load(even, i0 + 2 * stride);
+    work(odd, i0 + stride);
   }
   // the new token's row takes its slot (this step reads it from the input)
   if (hi == rows.count && hg == 0 && wave == kWaves - 1 && group == 0) {
-    const int64_t slot = rows.slot(last);
+    const int slot = rows.slot(last);
     const typename F::Frag kf = load_row<T, kVec>(new_k, d, a.dim), vf = load_row<T, kVec>(new_v, d, a.dim);
     float kx[E], vx[E];
 #pragma unroll
@@ -237,8 +301,8 @@ __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(StepCall a
       kx[e] = element<T>(kf, e);
       vx[e] = element<T>(vf, e);
     }
-    store_piece<T, kVec>(cache_k + slot * a.ck_slot, d, a.dim, kx);
-    store_piece<T, kVec>(cache_v + slot * a.cv_slot, d, a.dim, vx);
+    store_piece<T, kVec>(row_at(cache_k, slot, a.ck_slot), d, a.dim, kx);
+    store_piece<T, kVec>(row_at(cache_v, slot, a.cv_slot), d, a.dim, vx);
   }
 
 #pragma unroll
@@ -285,36 +349,49 @@ __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(StepCall a
   }
 }
 
-// Joins the parts of a row's walk: one wave per row and head.
+// Joins the parts of a row's walk: one block per row and head, whose waves take
+// every eighth part, all of their loads on their way at once.
 template <typename T>
-__global__ __launch_bounds__(kStepThreads) void attention_step_join_kernel(StepCall a, T* out) {
-  const int64_t at = (int64_t)blockIdx.x * (kStepThreads / kWave) + threadIdx.x / kWave;
-  if (at >= (int64_t)a.batch * a.q_heads) return;
-  const int64_t n = a.positions[at / a.q_heads];
+__global__ __launch_bounds__(kJoinThreads) void attention_step_join_kernel(StepCall a, T* out) {
+  constexpr int kWaves = kJoinThreads / kWave;
+  __shared__ float joined[kWaves][2 + 2 * kWave];
+  const int64_t at = blockIdx.x;
+  const int64_t n = load_uniform(a.positions + blockIdx.x / a.q_heads);
   if (n < 0) return;
   const StepRows rows(a, n);
-  const int64_t per = rows.per_part(a.parts);
-  const int parts = (int)((rows.count + per - 1) / per);
-  const float* p = a.part + at * a.parts * (2 + a.dim);
+  const int per = rows.per_part(a.parts);
+  const int parts = (rows.count + per - 1) / per, size = 2 + a.dim;
+  const float* p = a.part + at * a.parts * size;
+  const int wave = wave_id(), lane = lane_id();
   float m = kNoScore;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, p[(int64_t)i * (2 + a.dim)]);
+  for (int i = lane; i < parts; i += kWave) m = fmaxf(m, p[(int64_t)i * size]);
+  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
   float l = 0.f, v[2] = {0.f, 0.f};
-  for (int i = 0; i < parts; ++i) {
-    const float* x = p + (int64_t)i * (2 + a.dim);
+#pragma unroll 16
+  for (int i = wave; i < parts; i += kWaves) {
+    const float* x = p + (int64_t)i * size;
     const float f = exp2_fast(x[0] - m);
     l += x[1] * f;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      if (lane_id() + kWave * c < a.dim) v[c] += x[2 + lane_id() + kWave * c] * f;
+      if (lane + kWave * c < a.dim) v[c] += x[2 + lane + kWave * c] * f;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (lane == 0) joined[wave][0] = l;
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (lane_id() + kWave * c < a.dim) {
-      const float o = v[c] * inv;
-      if constexpr (sizeof(T) == 2) out[at * a.dim + lane_id() + kWave * c] = f32_to_bf16(o);
-      else out[at * a.dim + lane_id() + kWave * c] = o;
-    }
+  for (int c = 0; c < 2; ++c) joined[wave][2 + lane + kWave * c] = v[c];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= a.dim) return;
+  float o = 0.f;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    l += joined[w][0];
+    o += joined[w][2 + d];
+  }
+  o *= l > 0.f ? 1.f / l : 0.f;
+  if constexpr (sizeof(T) == 2) out[at * a.dim + d] = f32_to_bf16(o);
+  else out[at * a.dim + d] = o;
 }
 
 // The prompt form: rows of k and v at positions 0 .. length - 1 take their
@@ -333,12 +410,13 @@ __global__ __launch_bounds__(256) void cache_write_kernel(StepCall a, int64_t le
     const int64_t r = r0 + i / width, p = r - shift;
     const int c = (int)(i % width), kv = c / a.dim, d = c % a.dim;
     if (r >= len || p < 0 || p >= n) continue;
-    if (p >= a.sinks && p < n - a.ring) continue;
-    const int64_t slot = p < a.sinks ? p : a.sinks + (p - a.sinks) % a.ring;
+    const int ring = a.capacity - a.sinks;
+    if (p >= a.sinks && p < n - ring) continue;
+    const int64_t slot = p < a.sinks ? p : a.sinks + (p - a.sinks) % ring;
     static_cast<T*>(a.cache_k)[b * a.ck_batch + slot * a.ck_slot + kv * a.ck_head + d] =
-        static_cast<const T*>(a.k)[b * a.k_batch + r * a.q_batch + kv * a.k_head + d];
+        static_cast<const T*>(a.k)[b * a.k_batch + r * a.row_k + kv * a.k_head + d];
     static_cast<T*>(a.cache_v)[b * a.cv_batch + slot * a.cv_slot + kv * a.cv_head + d] =
-        static_cast<const T*>(a.v)[b * a.v_batch + r * a.q_head + kv * a.v_head + d];
+        static_cast<const T*>(a.v)[b * a.v_batch + r * a.row_v + kv * a.v_head + d];
   }
 }
 
@@ -377,6 +455,9 @@ int step_check(const mdl_attention_step* a, const char* what) {
     if (a->distances > kMaxDistances || a->num_buckets > 1024)
       return fail(MDL_ERR_UNSUPPORTED, w + ": bias buckets must begin at distances up to 2048, at most 1024 of them");
   }
+  if (a->capacity > 0x3fffffff || a->ck_slot < 0 || a->cv_slot < 0 || a->ck_slot > 0x7fffffff ||
+      a->cv_slot > 0x7fffffff)
+    return fail(MDL_ERR_UNSUPPORTED, w + ": at most 2^30 slots, less than 2^31 elements apart");
   if (a->batch > 0 && (!a->k || !a->v || !a->cache_k || !a->cache_v || !a->positions))
     return fail(MDL_ERR_INVALID, w + ": null pointer");
   return MDL_OK;
@@ -392,11 +473,11 @@ StepCall step_call(const mdl_attention_step& a) {
   c.q_batch = a.q_batch; c.q_head = a.q_head;
   c.k_batch = a.k_batch; c.k_head = a.k_head;
   c.v_batch = a.v_batch; c.v_head = a.v_head;
-  c.ck_batch = a.ck_batch; c.ck_slot = a.ck_slot; c.ck_head = a.ck_head;
-  c.cv_batch = a.cv_batch; c.cv_slot = a.cv_slot; c.cv_head = a.cv_head;
-  c.sinks = a.sinks;
-  c.ring = a.capacity - a.sinks;
-  c.window = a.window > 0 ? a.window : c.ring;
+  c.ck_batch = a.ck_batch; c.ck_slot = (uint32_t)a.ck_slot; c.ck_head = a.ck_head;
+  c.cv_batch = a.cv_batch; c.cv_slot = (uint32_t)a.cv_slot; c.cv_head = a.cv_head;
+  c.sinks = (int32_t)a.sinks;
+  c.capacity = (int32_t)a.capacity;
+  c.window = (int32_t)(a.window > 0 ? a.window : a.capacity - a.sinks);
   c.batch = (int32_t)a.batch; c.q_heads = a.q_heads; c.kv_heads = a.kv_heads; c.dim = a.head_dim;
   c.buckets = a.bias_table ? a.num_buckets : 0;
   c.distances = a.bias_table ? a.distances : 0;
@@ -415,19 +496,28 @@ bool step_vectors(const mdl_attention_step& a) {
          whole(a.cache_v, a.cv_batch, a.cv_slot, a.cv_head);
 }
 
+template <typename T, int L, int G, bool kVec, int kWaves>
+int launch_step(const StepCall& c, int64_t blocks, void* out, hipStream_t s) {
+  const size_t lds = ((size_t)c.buckets * G * 4 + (size_t)c.distances * 2 + 15) & ~size_t(15);
+  const auto kernel = attention_step_kernel<T, L, G, kVec, kWaves>;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * kWave), lds, s, c, static_cast<T*>(out));
+  MDL_CHECK_LAUNCH("attention_step_kernel");
+  return MDL_OK;
+}
+
 template <typename T, int L, int G, bool kVec>
-int launch_step(const StepCall& c, void* out, hipStream_t s) {
+int launch_step_blocks(const StepCall& c, void* out, hipStream_t s) {
   const int share = c.q_heads / c.kv_heads;
   const int64_t blocks = (int64_t)c.batch * c.kv_heads * ((share + G - 1) / G) * c.parts;
   if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_step: too many rows");
-  const size_t lds = ((size_t)c.buckets * G * 4 + (size_t)c.distances * 2 + 15) & ~size_t(15);
-  const auto kernel = attention_step_kernel<T, L, G, kVec>;
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kStepThreads), lds, s, c, static_cast<T*>(out));
-  MDL_CHECK_LAUNCH("attention_step_kernel");
+  if (int rc = blocks <= kFewBlocks ? launch_step<T, L, G, kVec, 8>(c, blocks, out, s)
+                                    : launch_step<T, L, G, kVec, 4>(c, blocks, out, s))
+    return rc;
   if (c.parts > 1) {
-    const int64_t joins = ((int64_t)c.batch * c.q_heads + kStepThreads / kWave - 1) / (kStepThreads / kWave);
-    hipLaunchKernelGGL(attention_step_join_kernel<T>, dim3((unsigned)joins), dim3(kStepThreads), 0, s, c,
+    const int64_t joins = (int64_t)c.batch * c.q_heads;
+    if (joins > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_step: too many rows");
+    hipLaunchKernelGGL(attention_step_join_kernel<T>, dim3((unsigned)joins), dim3(kJoinThreads), 0, s, c,
                        static_cast<T*>(out));
     MDL_CHECK_LAUNCH("attention_step_join_kernel");
   }
@@ -437,10 +527,10 @@ int launch_step(const StepCall& c, void* out, hipStream_t s) {
 template <typename T, int L, bool kVec>
 int launch_step_heads(const StepCall& c, void* out, hipStream_t s) {
   switch (heads_together(c.q_heads / c.kv_heads)) {
-    case 1: return launch_step<T, L, 1, kVec>(c, out, s);
-    case 2: return launch_step<T, L, 2, kVec>(c, out, s);
-    case 4: return launch_step<T, L, 4, kVec>(c, out, s);
-    default: return launch_step<T, L, 8, kVec>(c, out, s);
+    case 1: return launch_step_blocks<T, L, 1, kVec>(c, out, s);
+    case 2: return launch_step_blocks<T, L, 2, kVec>(c, out, s);
+    case 4: return launch_step_blocks<T, L, 4, kVec>(c, out, s);
+    default: return launch_step_blocks<T, L, 8, kVec>(c, out, s);
   }
 }
 
@@ -499,8 +589,8 @@ int mdl_attention_cache_write(const mdl_attention_step* a, int64_t len, int64_t 
   if (a->batch > 65535 || (len + 63) / 64 > 0x7fffffff)
     return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_cache_write: too many rows");
   StepCall c = step_call(with);
-  c.q_batch = k_row;  // the prompt's row strides
-  c.q_head = v_row;
+  c.row_k = k_row;
+  c.row_v = v_row;
   const dim3 grid((unsigned)((len + 63) / 64), (unsigned)a->batch);
   if (a->dtype == MDL_BF16)
     hipLaunchKernelGGL(cache_write_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream), c, len, lengths,

@@ -7,6 +7,7 @@
 // one call.
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -24,8 +25,10 @@ using torch::autograd::variable_list;
 
 namespace {
 
-at::TensorOptions options_of(const Tensor& t, at::ScalarType type) {
-  return at::TensorOptions().dtype(type).device(t.device());
+// A new contiguous tensor on t's device (allocated without a dispatcher round
+// trip: a small training step makes a dozen of them).
+Tensor empty_on(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return Tensor(at::detail::empty_cuda(sizes, type, t.device(), std::nullopt));
 }
 
 // The last dimension contiguous (any strides over the others).
@@ -120,11 +123,11 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward_cuda(
       attention_args(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
   c10::DeviceGuard guard(q.device());
   void* stream = stream_of(q.device());
-  Tensor out = at::empty(q.sizes(), options_of(q, q.scalar_type()));
-  Tensor stats = need_backward ? at::empty({q.size(0), q.size(2), q.size(1), 2}, options_of(q, at::kFloat))
-                               : at::empty({0}, options_of(q, at::kFloat));
+  Tensor out = empty_on(q, q.sizes(), q.scalar_type());
+  Tensor stats = need_backward ? empty_on(q, {q.size(0), q.size(2), q.size(1), 2}, at::kFloat)
+                               : empty_on(q, {0}, at::kFloat);
   const size_t bytes = mdl_attention_prepared_bytes(&a.call);
-  Tensor prepared = at::empty({(int64_t)bytes}, options_of(q, at::kByte));
+  Tensor prepared = empty_on(q, {(int64_t)bytes}, at::kByte);
   check(mdl_attention_prepare(&a.call, prepared.data_ptr(), bytes, stream), "mdl_attention_prepare");
   check(mdl_attention_forward(&a.call, prepared.data_ptr(), out.data_ptr(),
                               need_backward ? static_cast<float*>(stats.data_ptr()) : nullptr, stream),
@@ -149,12 +152,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
   same_device(grad_out, q, "attention gradient");
   c10::DeviceGuard guard(q.device());
   const Tensor go = inner_contiguous(grad_out);
-  Tensor dq = at::empty(q.sizes(), options_of(q, q.scalar_type()));
-  Tensor dk = at::empty(k.sizes(), options_of(k, k.scalar_type()));
-  Tensor dv = at::empty(v.sizes(), options_of(v, v.scalar_type()));
+  Tensor dq = empty_on(q, q.sizes(), q.scalar_type());
+  Tensor dk = empty_on(k, k.sizes(), k.scalar_type());
+  Tensor dv = empty_on(v, v.sizes(), v.scalar_type());
   need_table = need_table && bias_table.has_value();
-  Tensor dtable = need_table ? at::empty(bias_table->sizes(), options_of(q, bias_table->scalar_type()))
-                             : at::empty({0}, options_of(q, q.scalar_type()));
+  Tensor dtable = need_table ? empty_on(q, bias_table->sizes(), bias_table->scalar_type())
+                             : empty_on(q, {0}, q.scalar_type());
   if (q.numel() == 0) {
     dk.zero_();
     dv.zero_();
@@ -169,7 +172,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
   g.grad_q = dq.data_ptr(); g.grad_k = dk.data_ptr(); g.grad_v = dv.data_ptr();
   g.grad_table = need_table ? dtable.data_ptr() : nullptr;
   const size_t bytes = mdl_attention_backward_workspace_bytes(&a.call);
-  Tensor ws = workspace(bytes, q.device());
+  Tensor ws = empty_on(q, {(int64_t)bytes}, at::kByte);
   check(mdl_attention_backward(&a.call, prepared.data_ptr(), &g, ws.data_ptr(), bytes, stream_of(q.device())),
         "mdl_attention_backward");
   return {dq, dk, dv, dtable};
@@ -308,11 +311,11 @@ Tensor cache_step_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const 
   a.window = window;
   a.scale = (float)scale;
   c10::DeviceGuard guard(q.device());
-  Tensor out = at::empty(q.sizes(), options_of(q, q.scalar_type()));
+  Tensor out = empty_on(q, q.sizes(), q.scalar_type());
   if (a.batch == 0) return out;
   const size_t bytes = mdl_attention_step_workspace_bytes(&a);
   Tensor ws;
-  if (bytes) ws = workspace(bytes, q.device());
+  if (bytes) ws = empty_on(q, {(int64_t)bytes}, at::kByte);
   check(mdl_attention_step_forward(&a, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q.device())),
         "mdl_attention_step_forward");
   return out;
@@ -354,7 +357,7 @@ Tensor relative_bias_cuda(const Tensor& table, const Tensor& starts, bool bidire
   check_bias(table, starts, bidirectional, q_len, k_len);
   c10::DeviceGuard guard(table.device());
   const Tensor t = table.contiguous();
-  Tensor out = at::empty({t.size(1), q_len, k_len}, options_of(t, t.scalar_type()));
+  Tensor out = empty_on(t, {t.size(1), q_len, k_len}, t.scalar_type());
   check(mdl_relative_bias(t.data_ptr(), static_cast<const int32_t*>(starts.data_ptr()), (int32_t)t.size(0),
                           bidirectional, (int32_t)t.size(1), q_len, k_len, dtype_code(t.scalar_type()), out.data_ptr(),
                           stream_of(t.device())),
@@ -372,10 +375,10 @@ Tensor relative_bias_grad_cuda(const Tensor& grad, const Tensor& starts, int64_t
   const int32_t dtype = dtype_code(grad.scalar_type());
   c10::DeviceGuard guard(grad.device());
   const Tensor g = grad.contiguous();
-  Tensor out = at::empty({num_buckets, g.size(0)}, options_of(g, g.scalar_type()));
+  Tensor out = empty_on(g, {num_buckets, g.size(0)}, g.scalar_type());
   const size_t bytes =
       mdl_relative_bias_grad_workspace_bytes((int32_t)num_buckets, (int32_t)g.size(0), g.size(1), g.size(2), dtype);
-  Tensor ws = workspace(bytes, g.device());
+  Tensor ws = empty_on(g, {(int64_t)bytes}, at::kByte);
   check(mdl_relative_bias_grad(g.data_ptr(), static_cast<const int32_t*>(starts.data_ptr()), (int32_t)num_buckets,
                                bidirectional, (int32_t)g.size(0), g.size(1), g.size(2), dtype, out.data_ptr(),
                                ws.data_ptr(), bytes, stream_of(g.device())),
@@ -474,10 +477,10 @@ std::tuple<Tensor, Tensor, Tensor> block_norm_forward_cuda(
     double eps) {
   NormArgs a = norm_args(x, block_out, post_weight, next_weight, gate, residual_scale, eps);
   c10::DeviceGuard guard(x.device());
-  Tensor y = a.o.defined() ? at::empty(x.sizes(), options_of(x, x.scalar_type()))
-                           : at::empty({0}, options_of(x, x.scalar_type()));
-  Tensor h = at::empty(x.sizes(), options_of(x, x.scalar_type()));
-  Tensor rstd = at::empty({2, a.call.rows}, options_of(x, at::kFloat));
+  Tensor y = a.o.defined() ? empty_on(x, x.sizes(), x.scalar_type())
+                           : empty_on(x, {0}, x.scalar_type());
+  Tensor h = empty_on(x, x.sizes(), x.scalar_type());
+  Tensor rstd = empty_on(x, {2, a.call.rows}, at::kFloat);
   if (a.call.rows == 0) return {y, h, rstd};
   a.call.rstd = static_cast<float*>(rstd.data_ptr());
   check(mdl_block_norm_forward(&a.call, a.o.defined() ? y.data_ptr() : nullptr, h.data_ptr(), stream_of(x.device())),
@@ -507,10 +510,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> block_norm_backward_c
   dy = incoming(grad_y);
   dh = incoming(grad_h);
   auto like_x = [&](bool want) {
-    return want ? at::empty(x.sizes(), options_of(x, x.scalar_type())) : at::empty({0}, options_of(x, x.scalar_type()));
+    return want ? empty_on(x, x.sizes(), x.scalar_type()) : empty_on(x, {0}, x.scalar_type());
   };
   auto like_w = [&](bool want) {
-    return at::empty({want ? (int64_t)a.call.dim : 0}, options_of(x, next_weight.scalar_type()));
+    return empty_on(x, {want ? (int64_t)a.call.dim : 0}, next_weight.scalar_type());
   };
   Tensor dx = like_x(true), d_o = like_x(a.o.defined()), dgate = like_x(a.gate.defined());
   Tensor dscale = like_w(a.scale.defined() && (needs & 1)), dpost = like_w(a.post.defined() && (needs & 2)),
@@ -521,7 +524,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> block_norm_backward_c
   g.grad_x = ptr(dx); g.grad_block_out = ptr(d_o); g.grad_gate = ptr(dgate);
   g.grad_residual_scale = ptr(dscale); g.grad_post_weight = ptr(dpost); g.grad_next_weight = ptr(dnext);
   const size_t bytes = mdl_block_norm_backward_workspace_bytes(&a.call);
-  Tensor ws = workspace(bytes, x.device());
+  Tensor ws = empty_on(x, {(int64_t)bytes}, at::kByte);
   check(mdl_block_norm_backward(&a.call, &g, ws.data_ptr(), bytes, stream_of(x.device())), "mdl_block_norm_backward");
   return {dx, d_o, dgate, dscale, dpost, dnext};
 }
@@ -632,4 +635,15 @@ TORCH_LIBRARY_IMPL(mdl_hip, CUDA, m) {
   m.impl("relative_position_bias_backward", &relative_bias_grad_cuda);
   m.impl("block_norm_forward", &block_norm_forward_cuda);
   m.impl("block_norm_backward", &block_norm_backward_cuda);
+}
+
+// Inference: nothing to differentiate, and no call of the dispatcher's boxed
+// fallback for a missing autograd kernel.
+TORCH_LIBRARY_IMPL(mdl_hip, Autograd, m) {
+  m.impl("history_cache_step", torch::CppFunction::makeFallthrough());
+  m.impl("history_cache_write_", torch::CppFunction::makeFallthrough());
+}
+TORCH_LIBRARY_IMPL(mdl_hip, ADInplaceOrView, m) {
+  m.impl("history_cache_step", torch::CppFunction::makeFallthrough());
+  m.impl("history_cache_write_", torch::CppFunction::makeFallthrough());
 }

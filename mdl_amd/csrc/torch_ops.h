@@ -12,7 +12,5 @@ void* stream_of(const at::Device& d);
 // MDL_F32 / MDL_BF16; a TypeError for any other type.
 int dtype_code(at::ScalarType t);
 void require_device(const at::Tensor& t, const char* what);
-// Bytes of device memory.
-at::Tensor workspace(size_t bytes, const at::Device& dev);
 
 }  // namespace mdl_torch

@@ -35,6 +35,12 @@ from torch import Tensor
 from . import library  # noqa: F401  (loads libmdl_torch.so and its schemas)
 from .library import _cpu_kernel, _fake_kernel
 
+# the operators' overloads, looked up once
+_ATTENTION = torch.ops.mdl_hip.history_attention.default
+_BIAS = torch.ops.mdl_hip.relative_position_bias.default
+_STEP = torch.ops.mdl_hip.history_cache_step.default
+_WRITE = torch.ops.mdl_hip.history_cache_write_.default
+
 MAX_BUCKET_START = 2048
 MAX_BUCKETS = 1024
 
@@ -466,8 +472,7 @@ def history_attention(
     starts, distances = _bias_arguments(bias_table, buckets)
     if scale is None:
         scale = q.size(-1) ** -0.5 if q.ndim else 1.0
-    return torch.ops.mdl_hip.history_attention(q, k, v, mask, bias_table, starts, distances, _window_argument(window),
-                                               int(sinks), float(scale))
+    return _ATTENTION(q, k, v, mask, bias_table, starts, distances, _window_argument(window), int(sinks), float(scale))
 
 
 def relative_position_bias(table: Tensor, q_len: int, k_len: int, buckets: RelativeBuckets) -> Tensor:
@@ -477,8 +482,7 @@ def relative_position_bias(table: Tensor, q_len: int, k_len: int, buckets: Relat
 
     if table.ndim != 2 or table.size(0) != buckets.num_buckets:
         raise ValueError(f"bias table must have one row for each of the {buckets.num_buckets} buckets")
-    return torch.ops.mdl_hip.relative_position_bias(table, buckets.starts_on(table.device), buckets.bidirectional,
-                                                    int(q_len), int(k_len))
+    return _BIAS(table, buckets.starts_on(table.device), buckets.bidirectional, int(q_len), int(k_len))
 
 
 class HistoryCache:
@@ -517,15 +521,13 @@ class HistoryCache:
     def capacity(self) -> int:
         return self.k.size(1)
 
-    @torch.no_grad()
     def write(self, k: Tensor, v: Tensor, lengths: Tensor, *, right_aligned: bool = False) -> None:
         """Store prompts: ``k, v [B, L, Hkv, D]`` hold positions ``0 ..
         lengths[b] - 1`` of each row in their first rows, or in their last
         ones (``sequence_embedding_lookup``'s window) with ``right_aligned``."""
 
-        torch.ops.mdl_hip.history_cache_write_(k, v, self.k, self.v, lengths, self.sinks, right_aligned)
+        _WRITE(k, v, self.k, self.v, lengths, self.sinks, right_aligned)
 
-    @torch.no_grad()
     def step(self, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, *, bias_table: Optional[Tensor] = None,
              buckets: Optional[RelativeBuckets] = None, scale: Optional[float] = None) -> Tensor:
         """Store one new token a row and attend from it.
@@ -539,5 +541,5 @@ class HistoryCache:
         starts, distances = _bias_arguments(bias_table, buckets)
         if scale is None:
             scale = q.size(-1) ** -0.5
-        return torch.ops.mdl_hip.history_cache_step(q, k, v, self.k, self.v, positions, bias_table, starts, distances,
-                                                    self._window, self.sinks, float(scale))
+        return _STEP(q, k, v, self.k, self.v, positions, bias_table, starts, distances, self._window, self.sinks,
+                     float(scale))
