@@ -44,9 +44,15 @@ struct PrepareCall {
   float* bias;
   int64_t words_row;
   int32_t batch, k_len, heads, buckets, distances;
-  int32_t table_f32;
+  int32_t table_f32, mask_vec;  // mask_vec: mask rows in 16-byte pieces
   float inv_scale;
 };
+
+// The four bytes of x that are not 0, as four bits.
+__device__ __forceinline__ uint32_t byte_bits(uint32_t x) {
+  const uint32_t one = ((((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) >> 7) & 0x01010101u;
+  return (one * 0x01020408u) >> 24 & 15u;
+}
 
 __global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
   const int wave = threadIdx.x / kWave;
@@ -57,15 +63,40 @@ __global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
       const uint8_t* row = a.mask + block * a.mask_row;
       uint64_t* words = a.words + block * a.words_row;
       int first = a.k_len, last = -1;
-#pragma unroll 4
-      for (int w = wave; w < a.words_row; w += 4) {
-        const int col = 64 * w + lane_id();
-        const uint64_t word = __ballot(col < a.k_len && row[col] != 0);
-        if (word) {
-          if (first == a.k_len) first = 64 * w + __builtin_ctzll(word);
-          last = 64 * w + 63 - __builtin_clzll(word);
+      auto take = [&](int w, uint64_t word) {
+        if (!word) return;
+        if (first == a.k_len) first = 64 * w + __builtin_ctzll(word);
+        last = 64 * w + 63 - __builtin_clzll(word);
+      };
+      if (a.mask_vec) {
+        // a thread makes a word of its 64 columns' bytes
+        for (int w = threadIdx.x; w < a.words_row; w += 256) {
+          const int col = 64 * w;
+          uint64_t word = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (col + 16 * i < a.k_len) {
+              const u32x4 x = *(const gptr<u32x4>)(row + col + 16 * i);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) word |= (uint64_t)byte_bits(x[k]) << (16 * i + 4 * k);
+            }
+          words[w] = word;
+          take(w, word);
         }
-        if (lane_id() == 0) words[w] = word;
+      } else {
+        // a wave's lanes are the columns of a word
+#pragma unroll 4
+        for (int w = wave; w < a.words_row; w += 4) {
+          const int col = 64 * w + lane_id();
+          const uint64_t word = __ballot(col < a.k_len && row[col] != 0);
+          if (lane_id() == 0) words[w] = word;
+          take(w, word);
+        }
+      }
+      for (int s = 32; s >= 1; s >>= 1) {
+        const int f = __shfl_xor(first, s), l = __shfl_xor(last, s);
+        first = f < first ? f : first;
+        last = l > last ? l : last;
       }
       if (lane_id() == 0) {
         firsts[wave] = first;
@@ -374,6 +405,7 @@ int mdl_attention_prepare(const mdl_attention* a, void* prepared, size_t prepare
   PrepareCall c{};
   c.mask = a->mask;
   c.mask_row = a->mask_row;
+  c.mask_vec = reinterpret_cast<uintptr_t>(a->mask) % 16 == 0 && a->mask_row % 16 == 0 && a->k_len % 16 == 0;
   c.table = a->bias_table;
   c.starts = a->bucket_starts;
   c.words = reinterpret_cast<uint64_t*>(p + lay.words);

@@ -368,6 +368,12 @@ struct BlockBias {
   }
 };
 
+// A block without a pair: zeros for the heads' parts of the bias gradient.
+__device__ __forceinline__ void leave_nothing(const GradCall& g, int head, int heads, int64_t part) {
+  for (int i = threadIdx.x; i < heads * g.buckets; i += kAttnThreads)
+    g.bias_partial[((int64_t)(head + i / g.buckets) * g.bias_parts + part) * g.buckets + i % g.buckets] = 0.f;
+}
+
 // The pairs within a window: 128 keys a block, 32 per wave.
 template <typename T, int DP, bool kVec>
 __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCall a, GradCall g) {
@@ -393,19 +399,23 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   const uint32_t k_bits = mask.bits32(jw);
   const bool live = (k_bits >> l32) & 1;
 
-  KeyTile<T, DP> tile;
-  tile.template open<kVec>(a, b, kv, j, live);
-  const bool want_bias = g.bias_partial != nullptr;
-  BlockBias sums;
-  if (want_bias) sums.open(a, lds_bias + kStages * kBiasSpan, off - k0);
-  const int64_t part = (int64_t)b * key_blocks + kb;
-
   // columns of the queries with a pair here, as tiles of query rows
   int c_lo = k0 > mask.first ? k0 : mask.first, c_hi = k0 + kAttnRows - 1 + a.window - 1;
   if (c_hi > mask.last) c_hi = mask.last;
   if (c_lo < off) c_lo = off;
   const int t_first = (c_lo - off) / TQ;
-  const int per_head = c_lo <= c_hi && k0 <= mask.last ? (c_hi - off) / TQ - t_first + 1 : 0;
+  const bool any = c_lo <= c_hi && k0 <= mask.last && k0 + kAttnRows > mask.first;
+  const int per_head = any ? (c_hi - off) / TQ - t_first + 1 : 0;
+
+  KeyTile<T, DP> tile;
+  tile.template open<kVec>(a, b, kv, j, live);
+  const bool want_bias = g.bias_partial != nullptr;
+  const int64_t part = (int64_t)b * key_blocks + kb;
+  BlockBias sums;
+  if (want_bias) {
+    if (any) sums.open(a, lds_bias + kStages * kBiasSpan, off - k0);
+    else leave_nothing(g, kv * share, share, part);
+  }
 
   Stage qs, gs;
   int fetch_head = 0, fetch_tile = 0;  // the next pair to fetch: head of the group, tile of the walk
@@ -472,34 +482,51 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
     }
   };
   walk_tiles<kStages, 2 * Stage::kPer + 1, Stage::kDirect>(per_head * share, a.bias != nullptr, fetch, settle, work);
-  if (want_bias && per_head == 0)
-    for (int i = 0; i < share; ++i) sums.leave(a, g, kv * share + i, part);
-
-  if (j >= a.k_len) return;
-  if (g.far_partial) {
-    const int first = mask.first;
-    if (j >= first && j - first < a.sinks) {
-#pragma unroll 2
-      for (int n = 0; n < g.far_chunks; ++n) {
-        const float* far =
-            g.far_partial + (((((int64_t)b * a.kv_heads + kv) * g.far_chunks + n) * a.sinks + (j - first)) * 2) * a.dim;
+  // the far parts of the first tokens among the block's keys: summed over their
+  // chunks in order by all threads, 32 keys at a time, then taken from LDS
+  const int sink_end = mask.first + a.sinks < a.k_len ? mask.first + a.sinks : a.k_len;
+  if (g.far_partial && mask.first < k0 + kAttnRows && k0 < sink_end) {
+    float* summed = reinterpret_cast<float*>(smem);  // [32][2][dim]: no more than the tiles took
+    for (int w = 0; w < kAttnRows / 32; ++w) {
+      const int lo = k0 + 32 * w > mask.first ? k0 + 32 * w : mask.first;
+      const int hi = k0 + 32 * w + 32 < sink_end ? k0 + 32 * w + 32 : sink_end;
+      if (lo >= hi) continue;
+      __syncthreads();
+      const int n = (hi - lo) * 2 * a.dim;
+      const float* far = g.far_partial +
+                         (((int64_t)b * a.kv_heads + kv) * g.far_chunks * a.sinks + (lo - mask.first)) * 2 * a.dim;
+      const int64_t chunk = (int64_t)a.sinks * 2 * a.dim;
+      for (int i = threadIdx.x; i < n; i += kAttnThreads) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int c = 0; c < g.far_chunks; ++c) s += far[c * chunk + i];
+        summed[i] = s;
+      }
+      __syncthreads();
+      if (wave == w && j >= lo && j < hi) {
+        const float* mine = summed + (j - lo) * 2 * a.dim;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int d = 32 * dt + result_row(i);
             if (d < a.dim) {
-              tile.dk[dt][i] += far[d];
-              tile.dv[dt][i] += far[a.dim + d];
+              tile.dk[dt][i] += mine[d];
+              tile.dv[dt][i] += mine[a.dim + d];
             }
           }
       }
     }
   }
+  if (j >= a.k_len) return;
   const int64_t at = (((int64_t)b * a.k_len + j) * a.kv_heads + kv) * a.dim;
   store_result_row<T, DP>(static_cast<T*>(g.dk) + at, tile.dk, a.scale, a.dim);
   store_result_row<T, DP>(static_cast<T*>(g.dv) + at, tile.dv, 1.f, a.dim);
 }
+
+// Whether all pairs a window or more apart lie in the bias's last bucket: their
+// gradient is then one sum and needs none of the diagonals' LDS.
+__host__ __device__ __forceinline__ bool far_is_flat(const AttnCall& a) { return a.window >= a.distances - 1; }
 
 // Waves of a block that walk: those whose staged rows fit LDS beside the bias.
 template <typename T, int DP>
@@ -523,6 +550,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
   float* lr = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + kWalk * 64 * LD) + wave * (96 + kBias);
   float* lb = lr + 96;  // lr: (-m, -log2 sum)[32], -delta[32]
   float* joined = reinterpret_cast<float*>(smem);  // [dk, dv][32][dim], after the walk
+  __shared__ float flats[4];
 
   const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
   const int key_blocks = (a.sinks + 31) / 32;
@@ -537,15 +565,24 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
   const uint32_t k_bits = mask.bits32(k0) & low_bits(k_end - k0);
   const bool live = (k_bits >> l32) & 1;
 
+  const int64_t part = g.bias_far + ((int64_t)b * g.far_chunks + chunk) * key_blocks + kb;
+  const bool want_bias = g.bias_partial != nullptr;
+  float* to = g.far_partial + ((((int64_t)b * a.kv_heads + kv) * g.far_chunks + chunk) * a.sinks + 32 * kb) * 2 * a.dim;
+  const int r_first = chunk * kFarRows, r_last = r_first + kFarRows < a.q_len ? r_first + kFarRows : a.q_len;
+  if (k0 > mask.last || r_last - 1 + off < k0 + a.window || r_first + off > mask.last) {  // no pair
+    for (int i = threadIdx.x; i < 32 * 2 * a.dim; i += kAttnThreads)
+      if (32 * kb + i / (2 * a.dim) < a.sinks) to[i] = 0.f;
+    if (want_bias) leave_nothing(g, kv * share, share, part);
+    return;
+  }
+
   KeyTile<T, DP> tile;
   tile.template open<kVec>(a, b, kv, j, live);
-  const bool want_bias = g.bias_partial != nullptr;
   BlockBias sums;
-  if (want_bias)
+  const bool all_far = far_is_flat(a);
+  if (want_bias && !all_far)
     sums.open(a, reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + kWalk * 64 * LD) + kWalk * (96 + kBias), off - k0);
-  const int64_t part = g.bias_far + ((int64_t)b * g.far_chunks + chunk) * key_blocks + kb;
-
-  const int r_first = chunk * kFarRows, r_last = r_first + kFarRows < a.q_len ? r_first + kFarRows : a.q_len;
+  if (all_far) sums.diag.flat = 0.f;
   for (int hs = 0; hs < share; ++hs) {
     const int head = kv * share + hs;
     const float far_bias = a.bias ? load_uniform(head_bias(a, head) + kBiasEdge + a.distances - 1) : 0.f;
@@ -597,9 +634,22 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
       const uint32_t vis = live ? ~low_bits(j + a.window - col) & bits : 0u;
       const f32x16 ds =
           tile.add(lq, lg, lr, lr + 64, far_bias, far ? nullptr : lb + 31 - l32 + 4 * half, whole, vis, a.c2);
-      if (want_bias) sums.add(ds, corner, far);
+      if (want_bias) sums.add(ds, corner, far || all_far);
     }
-    if (want_bias) sums.leave(a, g, head, part);
+    if (!want_bias) continue;
+    if (!all_far) {
+      sums.leave(a, g, head, part);
+      continue;
+    }
+    float flat = sums.diag.flat;
+    for (int s = 32; s >= 1; s >>= 1) flat += __shfl_xor(flat, s);
+    sums.diag.flat = 0.f;
+    __syncthreads();
+    if (lane_id() == 0) flats[wave] = flat;
+    __syncthreads();
+    for (int k = threadIdx.x; k < g.buckets; k += kAttnThreads)
+      g.bias_partial[((int64_t)head * g.bias_parts + part) * g.buckets + k] =
+          k == g.buckets - 1 ? (flats[0] + flats[1]) + (flats[2] + flats[3]) : 0.f;
   }
 
   // the waves' sums, added in order
@@ -617,7 +667,6 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
     }
   }
   __syncthreads();
-  float* to = g.far_partial + ((((int64_t)b * a.kv_heads + kv) * g.far_chunks + chunk) * a.sinks + 32 * kb) * 2 * a.dim;
   for (int i = threadIdx.x; i < 32 * 2 * a.dim; i += kAttnThreads) {
     const int key = i / (2 * a.dim), which = i / a.dim & 1, d = i % a.dim;
     if (32 * kb + key < a.sinks) to[(int64_t)key * 2 * a.dim + which * a.dim + d] = joined[which * DP * 32 + d * 32 + key];
@@ -669,7 +718,8 @@ int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
   if (g.far_partial) {
     const int64_t blocks = key_unit_blocks(a, (a.sinks + 31) / 32 * g.far_chunks).blocks();
     const size_t walk =
-        far_waves<T, DP>() * ((size_t)64 * Tile<T, DP>::kLd * sizeof(T) + (96 + 64) * sizeof(float)) + bias_lds;
+        far_waves<T, DP>() * ((size_t)64 * Tile<T, DP>::kLd * sizeof(T) + (96 + 64) * sizeof(float)) +
+        (far_is_flat(a) ? 0 : bias_lds);
     const size_t join = (size_t)2 * DP * 32 * sizeof(float);
     const size_t lds = walk > join ? walk : join;
     const auto kernel = attention_grad_far_kernel<T, DP, kVec>;

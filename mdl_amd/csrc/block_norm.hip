@@ -50,6 +50,33 @@ struct NormRow {
 
   static __device__ __forceinline__ int column(int p) { return (p * L + (int)(threadIdx.x % L)) * E; }
 
+  // A row's pieces as they lie in memory: on their way while the row before is
+  // worked on.
+  struct Raw {
+    u32x4 piece[V];
+  };
+  static __device__ __forceinline__ void fetch(const void* base, int64_t row, int dim, Raw& r) {
+    const T* p = static_cast<const T*>(base) + row * dim;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      r.piece[i] = u32x4{0, 0, 0, 0};
+      if (column(i) < dim) r.piece[i] = ld_policy<kStream>(reinterpret_cast<const u32x4*>(p + column(i)));
+    }
+  }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 2) {
+          v[i * E + 2 * k] = __uint_as_float(r.piece[i][k] << 16);
+          v[i * E + 2 * k + 1] = __uint_as_float(r.piece[i][k] & 0xffff0000u);
+        } else {
+          v[i * E + k] = __uint_as_float(r.piece[i][k]);
+        }
+      }
+  }
+
   static __device__ __forceinline__ void load(const void* base, int64_t row, int dim, float (&v)[N]) {
     const T* p = static_cast<const T*>(base) + row * dim;
 #pragma unroll
@@ -199,20 +226,50 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormCall a)
 #pragma unroll
   for (int i = 0; i < N; ++i) d_scale[i] = d_post[i] = d_next[i] = 0.f;
   const float inv_dim = 1.f / (float)a.dim;
-  for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / L; row < a.rows;
-       row += (int64_t)gridDim.x * kGroups) {
-    float y[N], o[N], g[N], dx[N], dh[N];
-    Row::load(a.x, row, a.dim, y);
-    if (a.o) Row::load(a.o, row, a.dim, o);
-    if (a.gate) Row::load(a.gate, row, a.dim, g);
-    if (a.dh) Row::load(a.dh, row, a.dim, dh);
-    if (a.dy) {
-      Row::load(a.dy, row, a.dim, dx);
+  // the next row is read ahead where registers allow (8 elements a lane: 337 to
+  // 212 us for 262144 rows of 256 in bf16)
+  constexpr bool kAhead = kVec && N <= 8;
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  struct Rows {
+    typename Row::Raw x, o, g, dy, dh;
+    float inv_o, inv_y;
+  } next;
+  auto fetch = [&](int64_t row) {
+    Row::fetch(a.x, row, a.dim, next.x);
+    if (a.o) Row::fetch(a.o, row, a.dim, next.o);
+    if (a.gate) Row::fetch(a.gate, row, a.dim, next.g);
+    if (a.dh) Row::fetch(a.dh, row, a.dim, next.dh);
+    if (a.dy) Row::fetch(a.dy, row, a.dim, next.dy);
+    next.inv_o = a.o ? a.rstd[row] : 0.f;
+    next.inv_y = a.rstd[a.rows + row];
+  };
+  const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / L;
+  if constexpr (kAhead)
+    if (first < a.rows) fetch(first);
+  for (int64_t row = first; row < a.rows; row += step) {
+    float y[N], o[N], g[N], dx[N], dh[N], inv_o, inv_y;
+    if constexpr (kAhead) {
+      Row::unpack(next.x, y);
+      if (a.o) Row::unpack(next.o, o);
+      if (a.gate) Row::unpack(next.g, g);
+      if (a.dh) Row::unpack(next.dh, dh);
+      if (a.dy) Row::unpack(next.dy, dx);
+      inv_o = next.inv_o;
+      inv_y = next.inv_y;
+      if (row + step < a.rows) fetch(row + step);
     } else {
+      Row::load(a.x, row, a.dim, y);
+      if (a.o) Row::load(a.o, row, a.dim, o);
+      if (a.gate) Row::load(a.gate, row, a.dim, g);
+      if (a.dh) Row::load(a.dh, row, a.dim, dh);
+      if (a.dy) Row::load(a.dy, row, a.dim, dx);
+      inv_o = a.o ? a.rstd[row] : 0.f;
+      inv_y = a.rstd[a.rows + row];
+    }
+    if (!a.dy) {
 #pragma unroll
       for (int i = 0; i < N; ++i) dx[i] = 0.f;
     }
-    const float inv_o = a.o ? a.rstd[row] : 0.f, inv_y = a.rstd[a.rows + row];
     if (a.o) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
