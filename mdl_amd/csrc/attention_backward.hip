@@ -40,6 +40,14 @@ constexpr int kSpare = 96;      // distances of one tile and wave past either en
 constexpr int kFarRows = 256;   // query rows of a block of the first tokens' far part
 constexpr int kSkew = 64;       // diagonals of a 32x32 product tile, padded
 
+// Whether dP is computed alone and delta taken off it afterwards, instead of
+// dP starting there (one instruction less).  In fp32 the difference is then exact
+// where the two are close, and dP the same in every kernel: a row that sees one
+// key has dS = 0 to the bit, and sums of dS over such rows (the first of every
+// history) stay 0.  bf16 results do not resolve that.
+template <typename T>
+constexpr bool late_delta() { return sizeof(T) == 4; }
+
 // ------------------------------------------------------ queries: dq, delta --
 
 template <typename T, int DP, bool kVec>
@@ -127,7 +135,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
                        wc_lo + 31 - j0 < a.window;
 #pragma unroll
     for (int s = 0; s < kSubs; ++s) {
-      f32x16 x, dp = (f32x16)(-delta);
+      f32x16 x, dp = (f32x16)(late_delta<T>() ? 0.f : -delta);
       if (far) {
         x = (f32x16)(far_from);
       } else {
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, ll_neg));
-        dp[i] *= x[i];
+        dp[i] = (late_delta<T>() ? dp[i] - delta : dp[i]) * x[i];
         rest += dp[i];
       }
       // p and dS take the element type for the products with k
@@ -279,7 +287,7 @@ struct KeyTile {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       x[i] = stats[2 * (8 * (i >> 2) + (i & 3))];
-      dp[i] = delta[8 * (i >> 2) + (i & 3)];
+      dp[i] = late_delta<T>() ? 0.f : delta[8 * (i >> 2) + (i & 3)];
     }
     if (near_bias) {
 #pragma unroll
@@ -305,7 +313,7 @@ struct KeyTile {
     for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], c2, stats[2 * (8 * (i >> 2) + (i & 3)) + 1]));
     gt.times(x, dv);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= dp[i];
+    for (int i = 0; i < 16; ++i) x[i] *= late_delta<T>() ? dp[i] + delta[8 * (i >> 2) + (i & 3)] : dp[i];
     qt.times(x, dk);
     return x;
   }
