@@ -135,18 +135,17 @@ def norm(x, o, w_post, w_next, gate, scale, eps, dy=None, dh=None):
             (dx * sg * wp * n).sum(rows), (dx * sg * sc * n).sum(rows), dnext)
 
 
-def close(got, want, dtype, what="", terms=2):
-    """Norm-wise comparison.  A bfloat16 value is off by at most 2^-8 of itself;
-    a result passes at most ``terms`` such roundings (of the weights or their
-    gradients before a product, and of the result), each at most 2^-8 of the
-    norm.  fp32 sums of a few thousand products of unit size stay within
-    2^-24 sqrt(n) of theirs, below 1e-5.  The floor is that of a result whose
-    terms cancel: the same shares of unit terms."""
+def close(got, want, dtype, what="", fp32=1e-5):
+    """Norm-wise comparison.  A bfloat16 rounding moves a value by at most 2^-9
+    of itself, and a result passes at most four of them (inputs of its last
+    product and of the one before, a statistic, the result), so it is within
+    4 x 2^-9 of the norm.  fp32 sums of a few thousand products of unit size
+    stay within 2^-24 sqrt(n) of theirs, below 1e-5.  The norm counts at least as
+    0.1 an element: results whose unit terms cancel keep the terms' errors."""
 
-    tol = terms * 2.0 ** -8 if dtype == torch.bfloat16 else 1e-5
+    tol = 4 * 2.0 ** -9 if dtype == torch.bfloat16 else fp32
     got, want = got.double().cpu(), want.double().cpu()
     assert got.shape == want.shape, (what, got.shape, want.shape)
     assert torch.isfinite(got).all(), what
-    floor = 0.02 * math.sqrt(max(want.numel(), 1))
     error = float((got - want).norm())
-    assert error <= tol * (float(want.norm()) + floor), (what, error, float(want.norm()))
+    assert error <= tol * (float(want.norm()) + 0.1 * math.sqrt(want.numel())), (what, error, float(want.norm()))
