@@ -8,19 +8,28 @@
 // walks every (groups of the block)-th row with its own running maximum and
 // sum; groups, then waves, then blocks are joined at the end.  Few rows with
 // long caches are cut into parts over several blocks, joined by a second
-// launch.
+// launch.  256 users with up to 1028 rows of 64 (103 MB): 27.8 us, 3.7 TB/s, the
+// longest walks bound it; two users with 62,000 rows of 128 (129 MB): 26 and
+// 4 us, 4.2 TB/s together.
 #include "attention.cuh"
 
 namespace mdl {
 
-constexpr int kJoinThreads = 512;
-constexpr int kStepBlocks = 512;   // blocks wanted before a row's walk is no longer cut
-constexpr int kStepMinRows = 512;  // cached rows of a part at least
+constexpr int kJoinThreads = 1024;
+// A walk is cut where few of them would leave CUs idle; joining the parts
+// costs a launch of 4 to 5 us.  (bf16 caches of 1028 rows of 64, 8 query
+// heads on 2 key heads: one user 17 us whole, 16.5 in parts of 512 rows, 13.8
+// in four of 257; 100 users, 200 walks: 18.5 whole, 24.6 in two.)
+constexpr int kStepBlocks = 512;   // blocks wanted of walks that are cut
+constexpr int kCutUnits = 128;     // walks above which none is cut
+constexpr int kStepMinRows = 256;  // cached rows of a part at least
 
 // Rows of a lane group's iteration: twice as many are in flight (the next
-// iteration's are read while this one's are worked on).
+// iteration's are read while this one's are worked on).  The more heads share
+// a row, the fewer rows fill the registers (4 heads, 2 x 62,000 rows of 128:
+// 30.9 us with one, 32.7 with two).
 template <int G>
-constexpr int step_unroll() { return G == 8 ? 2 : 4; }
+constexpr int step_unroll() { return G == 8 ? 2 : (G == 4 ? 1 : 4); }
 
 struct StepCall {
   const void *q, *k, *v;
@@ -138,10 +147,13 @@ __device__ __forceinline__ void store_piece(T* row, int d, int D, const float* v
     }
 }
 
-// Waves of a block: four, so that several blocks share a CU; eight for calls
-// of at most a block per CU, which end with their one walk (one user's token
-// over 260 rows, 4 heads of 64: 8.7 us with four, 7.0 with eight).
-constexpr int kFewBlocks = 256;
+// Waves of a block: eight for calls of at most two blocks per CU (one with 8
+// heads' registers), which end with their longest walk; four where further
+// blocks wait for a CU.  (One user's token over 260 rows, 4 heads of 64: 8.7 us
+// with four, 7.3 with eight.  512 walks of up to 1028 rows, 4 heads a row: 30.4
+// and 27.8; 4096 such walks: 166 and 186.)
+template <int G>
+constexpr int few_blocks() { return G == 8 ? 256 : 512; }
 
 template <typename T, int L, int G, bool kVec, int kWaves>
 __global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall a, T* out) {
@@ -349,11 +361,13 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall 
   }
 }
 
-// Joins the parts of a row's walk: one block per row and head, whose waves take
-// every eighth part, all of their loads on their way at once.
+// Joins the parts of a row's walk: one block per row and head.  Waves take every
+// kWaves-th part, kAtOnce of them with all loads on their way at once and no
+// load waiting for a maximum: the parts come from other XCDs, a trip of about
+// a microsecond (128 parts of 16 rows: 4.2 us; 13 with the maximum first).
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void attention_step_join_kernel(StepCall a, T* out) {
-  constexpr int kWaves = kJoinThreads / kWave;
+  constexpr int kWaves = kJoinThreads / kWave, kAtOnce = 8;
   __shared__ float joined[kWaves][2 + 2 * kWave];
   const int64_t at = blockIdx.x;
   const int64_t n = load_uniform(a.positions + blockIdx.x / a.q_heads);
@@ -363,31 +377,55 @@ __global__ __launch_bounds__(kJoinThreads) void attention_step_join_kernel(StepC
   const int parts = (rows.count + per - 1) / per, size = 2 + a.dim;
   const float* p = a.part + at * a.parts * size;
   const int wave = wave_id(), lane = lane_id();
-  float m = kNoScore;
-  for (int i = lane; i < parts; i += kWave) m = fmaxf(m, p[(int64_t)i * size]);
-  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  float l = 0.f, v[2] = {0.f, 0.f};
-#pragma unroll 16
-  for (int i = wave; i < parts; i += kWaves) {
-    const float* x = p + (int64_t)i * size;
-    const float f = exp2_fast(x[0] - m);
-    l += x[1] * f;
+  // a lane's two dimensions; those past the last take its value and are not stored
+  const int d0 = lane < a.dim ? lane : a.dim - 1, d1 = lane + kWave < a.dim ? lane + kWave : a.dim - 1;
+  float m = kNoScore, l = 0.f, v0 = 0.f, v1 = 0.f;
+  for (int i0 = wave; i0 < parts; i0 += kWaves * kAtOnce) {
+    float pm[kAtOnce], pl[kAtOnce], p0[kAtOnce], p1[kAtOnce];
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      if (lane + kWave * c < a.dim) v[c] += x[2 + lane + kWave * c] * f;
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * kWaves;
+      const float* x = p + (int64_t)(i < parts ? i : i0) * size;
+      pm[u] = x[0];
+      pl[u] = x[1];
+      p0[u] = x[2 + d0];
+      p1[u] = x[2 + d1];
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) top = fmaxf(top, pm[u]);
+    const float f = exp2_fast(m - top);
+    m = top;
+    l *= f;
+    v0 *= f;
+    v1 *= f;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float w = i0 + u * kWaves < parts ? exp2_fast(pm[u] - m) : 0.f;
+      l = __builtin_fmaf(pl[u], w, l);
+      v0 = __builtin_fmaf(p0[u], w, v0);
+      v1 = __builtin_fmaf(p1[u], w, v1);
+    }
   }
-  if (lane == 0) joined[wave][0] = l;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) joined[wave][2 + lane + kWave * c] = v[c];
+  if (lane == 0) {
+    joined[wave][0] = m;
+    joined[wave][1] = l;
+  }
+  joined[wave][2 + lane] = v0;
+  joined[wave][2 + kWave + lane] = v1;
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= a.dim) return;
+  m = joined[0][0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, joined[w][0]);
   float o = 0.f;
   l = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    l += joined[w][0];
-    o += joined[w][2 + d];
+    const float f = exp2_fast(joined[w][0] - m);
+    l = __builtin_fmaf(joined[w][1], f, l);
+    o = __builtin_fmaf(joined[w][2 + d], f, o);
   }
   o *= l > 0.f ? 1.f / l : 0.f;
   if constexpr (sizeof(T) == 2) out[at * a.dim + d] = f32_to_bf16(o);
@@ -424,14 +462,15 @@ __global__ __launch_bounds__(256) void cache_write_kernel(StepCall a, int64_t le
 
 int heads_together(int share) { return share >= 5 ? 8 : (share >= 3 ? 4 : share); }
 
-// Blocks that share a row's walk: as many as fill the card, each with
-// kStepMinRows cached rows at least.
+// Blocks that share a row's walk: one, unless the walks leave half of the CUs
+// idle; then as many as give each CU two, of kStepMinRows cached rows or more.
 int step_parts(const mdl_attention_step& a) {
   const int share = a.q_heads / a.kv_heads, g = heads_together(share);
   const int64_t units = a.batch * a.kv_heads * ((share + g - 1) / g);
+  if (units > kCutUnits) return 1;
   const int64_t most = a.window > 0 && a.window + a.sinks < a.capacity ? a.window + a.sinks : a.capacity;
-  int64_t parts = (kStepBlocks + units - 1) / (units > 0 ? units : 1);
-  const int64_t cap = (most + kStepMinRows - 1) / kStepMinRows;
+  int64_t parts = kStepBlocks / (units > 0 ? units : 1);
+  const int64_t cap = most / kStepMinRows;
   if (parts > cap) parts = cap;
   return parts < 1 ? 1 : (int)parts;
 }
@@ -511,7 +550,7 @@ int launch_step_blocks(const StepCall& c, void* out, hipStream_t s) {
   const int share = c.q_heads / c.kv_heads;
   const int64_t blocks = (int64_t)c.batch * c.kv_heads * ((share + G - 1) / G) * c.parts;
   if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_step: too many rows");
-  if (int rc = blocks <= kFewBlocks ? launch_step<T, L, G, kVec, 8>(c, blocks, out, s)
+  if (int rc = blocks <= few_blocks<G>() ? launch_step<T, L, G, kVec, 8>(c, blocks, out, s)
                                     : launch_step<T, L, G, kVec, 4>(c, blocks, out, s))
     return rc;
   if (c.parts > 1) {
