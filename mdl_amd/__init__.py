@@ -12,6 +12,7 @@ kernels in ``libmdl_hip.so`` behind the reference's Python API:
 * :mod:`mdl_amd.sparse_step` -- one fused forward + backward + update step;
 * :mod:`mdl_amd.history` -- attention over histories, training and serving;
 * :mod:`mdl_amd.block_norm` -- the norms around a block with its gate and residual scale;
+* :mod:`mdl_amd.history_encoder` -- an encoder of histories on these operators;
 * :mod:`mdl_amd.ops` -- tensor-level calls of the C ABI (include/mdl_hip.h);
 * :mod:`mdl_amd.library` -- the same path as ``torch.library`` custom ops
   (``torch.ops.mdl_hip.*``, registered when the package is imported).

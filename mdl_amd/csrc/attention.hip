@@ -7,6 +7,15 @@
 // are the result's columns, so a query's statistics are one value per lane),
 // p = exp2(c2 x - c2 m), and out^T += V^T p^T.  Out is divided by l at the
 // end; a query without a visible key gets zeros.
+//
+// The products' operands come from LDS (24 KB a wave and 32 x 64 scores of head
+// dimension 128), where rows lie for both readings without bank conflicts, and
+// tile t + 1 is on its way while tile t is worked on.  What bounds it: the wave's
+// own chain of products, exponentials (a quarter of the vector rate) and
+// products; matrix instructions are busy about half of the time at dimension
+// 128 (8192 rows, window 1024, 16 heads: 230 us, 600 TFLOP/s) and a third at 64,
+// where a 256-key window's tiles are mostly masked (64 ragged rows of 2048:
+// 90 us).  Taking instructions out (constant starts, masks) changed little.
 #include "attention.cuh"
 
 namespace mdl {
@@ -135,8 +144,10 @@ __global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
 // (p stays below 2^8): most tiles then skip the rescaling of out.
 constexpr float kLazyRaise = 8.f;
 
-// Two waves more than the two that most registers would allow hide the
-// latencies of bf16's narrow tiles better than reading ahead.
+// Waves a SIMD that the registers are held to.  The narrow tiles of bf16 are
+// short of work between their waits: three waves instead of the two that free
+// registers would give took 64 x 2048 rows (4 heads of 64, window 256) from 105
+// to 90 us and 8 x 4096 without a window (8 heads on 2) from 195 to 180.
 template <typename T, int DP>
 constexpr int forward_waves() { return sizeof(T) == 2 && DP <= 64 ? 3 : 1; }
 
@@ -180,7 +191,7 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
   for (int i = 0; i < DP / 32; ++i) acc[i] = (f32x16)(0.f);
   float m = kNoScore, mneg = -(kNoScore * a.c2), l = 0.f;
   const float lazy = kLazyRaise / a.c2;
-  const f32x16 far_bias = (f32x16)(bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f);
+  const float far_bias = bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f;
 
   const Tile<T, DP> read;
   Stage ks, vs;
@@ -198,6 +209,7 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
     ks.settle(lds + slot * 2 * TK * LD);
     vs.settle(lds + slot * 2 * TK * LD + TK * LD);
   };
+  auto large = [&](float most, float bias_of_all) { return is_large(a, fabsf(most) + fabsf(bias_of_all)); };
   auto work = [&](int i, int slot) {
     const T* lk = lds + slot * 2 * TK * LD;
     const T* lv = lk + TK * LD;
@@ -220,8 +232,9 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
     for (int s = 0; s < kSubs; ++s) {
       const NatFrags<T, DP> k(read, lk, s);
       if constexpr (DP > 64) reads_first<T>();
-      x[s] = far ? k.times(q, far_bias) : k.times(q, x[s]);
+      x[s] = far ? k.times(q, (f32x16)(0.f)) : k.times(q, x[s]);
     }
+    const float shift = far ? far_bias : 0.f;  // what x lacks: one bias for the tile is added to the maximum instead
     const TrFrags<T, DP> v0(read, lv, 0);
     const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
                        wc_lo + 31 - j0 < a.window;
@@ -239,7 +252,7 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
     for (int s = 0; s < kSubs; ++s)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, x[s][i]);
-    top = max_halves(top);
+    top = max_halves(top) + shift;
     if (__any(top > m + lazy)) {
       const float up = fmaxf(m, top);
       const float shrink = exp2_fast((m - up) * a.c2);
@@ -249,11 +262,18 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) acc[i] *= shrink;
     }
+    float from = __builtin_fmaf(shift, a.c2, mneg);
+    if (__any(large(m, shift))) {
+      const float add = large(m, shift) ? shift : 0.f, less = large(m, shift) ? m : 0.f;
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) x[s] = (x[s] + add) - less;
+      from = large(m, shift) ? 0.f : from;
+    }
     // the weights take the element type for the second product; their sum does not
     auto weigh = [&](f32x16& w) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        w[i] = exp2_fast(__builtin_fmaf(w[i], a.c2, mneg));
+        w[i] = exp2_fast(__builtin_fmaf(w[i], a.c2, from));
         l += w[i];
       }
     };
@@ -276,7 +296,7 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
     store_result_row<T, DP>(out + at, acc, inv, a.dim);
     if (stats && half == 0) {
       // -m and -log2 of the sum at the unrounded c2 m; -inf makes every weight of an empty row 0
-      const float ll = l > 0.f ? __builtin_fmaf(m, a.c2, mneg) - log2f(l) : -INFINITY;
+      const float ll = l > 0.f ? (large(m, 0.f) ? 0.f : __builtin_fmaf(m, a.c2, mneg)) - log2f(l) : -INFINITY;
       stats[((int64_t)b * a.q_heads + head) * a.q_len + row] = make_float2(l > 0.f ? -m : 0.f, ll);
     }
   }

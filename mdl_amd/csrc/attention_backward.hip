@@ -16,7 +16,17 @@
 // all the same, adds the row's dS in fp32 to what it is short of (their sum
 // is 0 with the true delta), and takes the share of k that belongs to the
 // difference (a fourth product, sum p k) off dq at the end; the second kernel
-// reads the corrected delta.
+// reads the corrected delta.  (The residual of out, saved by the forward, would
+// spare that product, 45 us of 490 at dimension 128, for another 2 bytes per
+// element of out held until the backward.)
+//
+// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 130 us for
+// the queries, 165 for the keys, 42 for the first tokens' far pairs; 2 x 8192
+// rows (16 heads of 128 on 4, window 1024): 485, 540 and 45.  At dimension 128
+// the accumulators leave room for one wave a SIMD, whose chain of LDS reads,
+// products and exponentials bounds it (matrix instructions 30 % of the time);
+// two waves spill (540 for the queries), and the products of one sub-tile under
+// the exponentials of another took longer (466 against 433, both without sum p k).
 #include "attention.cuh"
 
 namespace mdl {
@@ -106,7 +116,10 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = pk[i] = (f32x16)(0.f);
   float rest = 0.f;  // sum of dS: delta less dO . out
-  const float far_from = (bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f) + m_neg;
+  const float far_bias = bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f;
+  // scores start at the bias less the maximum; a large maximum is taken off at the end
+  const bool large = bias && is_large(a, m_neg), any_large = __any(large);
+  const float far_from = large ? 0.f : far_bias + m_neg, near_from = large ? 0.f : m_neg;
 
   const Tile<T, DP> read;
   Stage ks, vs;
@@ -132,7 +145,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
     const uint64_t bits = mask.bits<TK>(j0);
     const bool far = !bias || wc_lo - j1 >= a.distances - 1;
     const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
-                       wc_lo + 31 - j0 < a.window;
+                       wc_lo + 31 - j0 < a.window && !any_large;
 #pragma unroll
     for (int s = 0; s < kSubs; ++s) {
       f32x16 x, dp = (f32x16)(late_delta<T>() ? 0.f : -delta);
@@ -141,7 +154,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
       } else {
         const float* from = lds_bias + slot * kBiasSpan + (32 * wave + l32 + TK - 1 - 32 * s - 4 * half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = from[-(8 * (i >> 2) + (i & 3))] + m_neg;
+        for (int i = 0; i < 16; ++i) x[i] = from[-(8 * (i >> 2) + (i & 3))] + near_from;
       }
       {
         const NatFrags<T, DP> kn(read, lk, s), vn(read, lv, s);
@@ -152,6 +165,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
       const TrFrags<T, DP> kt(read, lk, s);
       reads_first<T>();
       if (!whole) {
+        if (any_large) x = (x + (far && large ? far_bias : 0.f)) + (large ? m_neg : 0.f);
         uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
         vis >>= 4 * half;
 #pragma unroll
@@ -279,8 +293,9 @@ struct KeyTile {
   // delta: theirs (-m and -log2 sum; -delta); near_bias: the pairs' biases
   // by row (NULL: all far_bias); vis: the visible rows of the lane's key.
   __device__ __forceinline__ f32x16 add(const T* q, const T* go, const float* stats, const float* delta, float far_bias,
-                                        const float* near_bias, bool whole, uint32_t vis, float c2) {
+                                        const float* near_bias, bool whole, uint32_t vis, const AttnCall& a) {
     const int half = lane_id() >> 5;
+    const bool any_large = a.bias && __any(is_large(a, stats[2 * (lane_id() & 31)]));
     stats += 8 * half;
     delta += 4 * half;
     f32x16 x, dp;
@@ -296,11 +311,23 @@ struct KeyTile {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] += far_bias;
     }
+    if (any_large) {  // rows with a large maximum start without it, and far ones without their bias
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (is_large(a, stats[2 * (8 * (i >> 2) + (i & 3))])) x[i] = near_bias ? near_bias[8 * (i >> 2) + (i & 3)] : 0.f;
+    }
     {
       const NatFrags<T, DP> qn(read, q, 0), gn(read, go, 0);
       reads_first<T>();
       x = qn.times(k, x);
       dp = gn.times(v, dp);
+    }
+    if (any_large) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float m_neg = stats[2 * (8 * (i >> 2) + (i & 3))];
+        if (is_large(a, m_neg)) x[i] = (x[i] + (near_bias ? 0.f : far_bias)) + m_neg;
+      }
     }
     const TrFrags<T, DP> gt(read, go, 0), qt(read, q, 0);
     reads_first<T>();
@@ -310,7 +337,7 @@ struct KeyTile {
       for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], c2, stats[2 * (8 * (i >> 2) + (i & 3)) + 1]));
+    for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, stats[2 * (8 * (i >> 2) + (i & 3)) + 1]));
     gt.times(x, dv);
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] *= late_delta<T>() ? dp[i] + delta[8 * (i >> 2) + (i & 3)] : dp[i];
@@ -477,7 +504,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
           vis = live ? ~low_bits(j - col) & low_bits(j + a.window - col) & (uint32_t)(bits >> (32 * s)) : 0u;
         const f32x16 ds =
             tile.add(lq + 32 * s * LD, lg + 32 * s * LD, lr + 64 * s, lr + 2 * TQ + 32 * s, far_bias,
-                     far ? nullptr : lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half), whole, vis, a.c2);
+                     far ? nullptr : lb + (kAttnRows - 1 - 32 * wave - l32 + 32 * s + 4 * half), whole, vis, a);
         if (want_bias) sums.add(ds, corner, far);
       }
     }
@@ -641,7 +668,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
       const bool whole = k_bits == ~0u && bits == ~0u && corner - 31 >= a.window;
       const uint32_t vis = live ? ~low_bits(j + a.window - col) & bits : 0u;
       const f32x16 ds =
-          tile.add(lq, lg, lr, lr + 64, far_bias, far ? nullptr : lb + 31 - l32 + 4 * half, whole, vis, a.c2);
+          tile.add(lq, lg, lr, lr + 64, far_bias, far ? nullptr : lb + 31 - l32 + 4 * half, whole, vis, a);
       if (want_bias) sums.add(ds, corner, far || all_far);
     }
     if (!want_bias) continue;

@@ -448,12 +448,6 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// *p += v in LDS, without a result.
-__device__ __forceinline__ void lds_add(float* p, float v) {
-  typedef __attribute__((address_space(3))) float* lds_float;
-  __builtin_amdgcn_ds_faddf((lds_float)p, v, 0, 0, false);
-}
-
 // The sum of v over this lane and the lane 32 away.
 __device__ __forceinline__ float sum_halves(float v) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

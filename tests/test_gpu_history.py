@@ -149,6 +149,33 @@ def test_bias_shuts_distances_out(device, dtype, low):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [-1e4, -3e6, -1e10, -1e20, "lowest"])
+def test_bias_of_mask_size_everywhere(device, dtype, low):
+    """Rows that see only biases meant as masks still answer an average of
+    their values: scores are added to the bias in fp32, where a bias of 1e10 or
+    more swallows them all (the mean), and one of 1e4 none of 0.01."""
+
+    announce("mask-size bias", dtype, low)
+    value = torch.finfo(dtype).min if low == "lowest" else low
+    q, k, v = (make(i, dtype, 2, 150, 2, 32, std=3.0 if i < 2 else 1.0) for i in range(3))
+    table = torch.full((8, 2), value, dtype=dtype)
+    leaves = [t.to(device).requires_grad_() for t in (q, k, v, table)]
+    out = history_attention(*leaves[:3], bias_table=leaves[3], buckets=RelativeBuckets(8, 24))
+    out.square().sum().backward()
+    assert all(torch.isfinite(t.grad).all() for t in leaves)
+    got = out.detach().double().cpu()
+    span = v.double().abs().cummax(1).values * (1 + 2.0 ** -8)
+    assert torch.isfinite(got).all() and (got.abs() <= span).all()
+    if low not in (-1e4, -3e6):
+        mean = v.double().cumsum(1) / torch.arange(1, 151)[:, None, None]
+        R.close(got, mean, dtype)
+    elif low == -1e4 and dtype == F32:
+        # scores next to 5.7e4 (the bias divided by the scale) are off by 2^-9, the weights by 2^-9 scale
+        want = R.attention(q, k, v, None, 0, 0, torch.zeros(8, 2), (8, 24))
+        R.close(got, want, dtype, fp32=2.0 ** -9)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("how", ["fused", "offset", "expanded", "heads_first", "grad"])
 def test_attention_strides(device, dtype, how):
     announce("strides", dtype, how)
