@@ -274,11 +274,16 @@ struct RowMask {
     if (s > 32) x |= load_uniform(words + w + 1) << (64 - s);
     return (uint32_t)x;
   }
+  // 64 columns (or 32) likewise
   template <int kTile>
   __device__ __forceinline__ uint64_t bits(int col) const {
-    const uint32_t lo = bits32(col);
-    if (kTile == 32) return lo;
-    return lo | (uint64_t)bits32(col + 32) << 32;
+    if (kTile == 32) return bits32(col);
+    if (!words) return low_bits(k_len - col) | (uint64_t)low_bits(k_len - col - 32) << 32;
+    if (col >= k_len) return 0;
+    const int w = col >> 6, s = col & 63;
+    uint64_t x = load_uniform(words + w) >> s;
+    if (s) x |= load_uniform(words + w + 1) << (64 - s);
+    return x;
   }
 };
 
@@ -325,13 +330,11 @@ __device__ __forceinline__ uint32_t lds_address(void* lds) {
   typedef __attribute__((address_space(3))) void* lds_void;
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void)lds);
 }
-__device__ __forceinline__ void copy16_to_lds(void* lds, const void* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_address(lds)), "v"(from)
-               : "memory");
+__device__ __forceinline__ void copy16_to_lds(uint32_t lds, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
 }
-__device__ __forceinline__ void copy4_to_lds(void* lds, const void* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_address(lds)), "v"(from)
-               : "memory");
+__device__ __forceinline__ void copy4_to_lds(uint32_t lds, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 
 // All but the wave's last kLeft memory operations have ended: the copies
@@ -359,23 +362,46 @@ struct TileStage {
   static constexpr int kPieces = DP / F::kElems;  // per row
   static constexpr int kPer = F::kTile * kPieces / kAttnThreads;
   static_assert(F::kTile * kPieces % kAttnThreads == 0, "whole pieces per thread");
+  static constexpr int kRows = kAttnThreads / kPieces;  // from a piece of a thread to its next
   typename F::Frag r[kDirect ? 1 : kPer];
+  const T* mine;    // the thread's first piece (direct) or row, in row 0 of base
+  int64_t stride;
+  uint32_t to;      // the wave's place in the first buffer
+  bool inside, full;
 
-  // rows row0 .. of base; bits: the live ones
-  __device__ __forceinline__ void fetch(T* lds, const T* base, int64_t stride, int row0, uint64_t bits, int D) {
+  // lds: the first of the buffers
+  __device__ __forceinline__ void open(T* lds, const T* base, int64_t row_stride, int D) {
+    stride = row_stride;
+    const int row = threadIdx.x / kPieces;
+    mine = base + row * stride;
+    full = D == DP;
+    if constexpr (kDirect) {
+      // the lane's place in LDS is given; the piece that belongs there is the same in each of its rows
+      static_assert(kRows % 16 == 0, "the swap's period");
+      const int d = ((threadIdx.x % kPieces) ^ Lds::swap(row)) * F::kElems;
+      mine += d;
+      inside = d < D;
+      to = lds_address(lds + wave_id() * kWave * F::kElems);
+    }
+  }
+  // A tile to the buffer `past` bytes after the first; first: elements from base
+  // to its first row; bits: the live ones.
+  __device__ __forceinline__ void fetch(uint32_t past, int64_t first, uint64_t bits, int D) {
+    const T* from = mine + first;
+    if (kDirect && full && bits == ~0ull) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) copy16_to_lds(to + past + i * kAttnThreads * 16, from + i * kRows * stride);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int idx = i * kAttnThreads + threadIdx.x;
-      const int row = idx / kPieces;
-      const bool live = (bits >> row) & 1;
+      const bool live = (bits >> (threadIdx.x / kPieces + i * kRows)) & 1;
+      const T* row = from + i * kRows * stride;
       if constexpr (kDirect) {
-        // the lane's place in LDS is given; the piece that belongs there
-        const int d = ((idx % kPieces) ^ Lds::swap(row)) * F::kElems;
-        const T* from = live && d < D ? base + (int64_t)(row0 + row) * stride + d : zero_row<T>();
-        copy16_to_lds(lds + (i * kAttnThreads + wave_id() * kWave) * F::kElems, from);
+        copy16_to_lds(to + past + i * kAttnThreads * 16, live && inside ? row : zero_row<T>());
       } else {
         r[i] = {};
-        if (live) r[i] = load_row<T, kVec>(base + (int64_t)(row0 + row) * stride, idx % kPieces * F::kElems, D);
+        if (live) r[i] = load_row<T, kVec>(row, threadIdx.x % kPieces * F::kElems, D);
       }
     }
   }

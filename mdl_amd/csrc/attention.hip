@@ -195,15 +195,18 @@ __global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attent
 
   const Tile<T, DP> read;
   Stage ks, vs;
+  ks.open(lds, kp, a.k_row, a.dim);
+  vs.open(lds + TK * LD, vp, a.v_row, a.dim);
+  const uint32_t bias_to = lds_address(lds_bias + wave * kWave);
   auto fetch = [&](int i, int slot) {
     const int j0 = walk.tile_at(i) * TK;
     const uint64_t bits = mask.bits<TK>(j0);
-    T* to = lds + slot * 2 * TK * LD;
-    ks.fetch(to, kp, a.k_row, j0, bits, a.dim);
-    vs.fetch(to + TK * LD, vp, a.v_row, j0, bits, a.dim);
+    const uint32_t past = slot * (2 * TK * LD * (uint32_t)sizeof(T));
+    ks.fetch(past, j0 * a.k_row, bits, a.dim);
+    vs.fetch(past, j0 * a.v_row, bits, a.dim);
     // lds_bias[i]: distance i + that of the block's first query and the tile's last key
     if (bias)
-      copy4_to_lds(lds_bias + slot * kBiasSpan + wave * kWave, bias + bias_at(a, r0 + off - j0 - (TK - 1)) + threadIdx.x);
+      copy4_to_lds(bias_to + slot * (kBiasSpan * 4), bias + bias_at(a, r0 + off - j0 - (TK - 1)) + threadIdx.x);
   };
   auto settle = [&](int slot) {
     ks.settle(lds + slot * 2 * TK * LD);

@@ -123,14 +123,17 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 
   const Tile<T, DP> read;
   Stage ks, vs;
+  ks.open(lds, kp, a.k_row, a.dim);
+  vs.open(lds + TK * LD, vp, a.v_row, a.dim);
+  const uint32_t bias_to = lds_address(lds_bias + wave * kWave);
   auto fetch = [&](int i, int slot) {
     const int j0 = walk.tile_at(i) * TK;
     const uint64_t bits = mask.bits<TK>(j0);
-    T* to = lds + slot * 2 * TK * LD;
-    ks.fetch(to, kp, a.k_row, j0, bits, a.dim);
-    vs.fetch(to + TK * LD, vp, a.v_row, j0, bits, a.dim);
+    const uint32_t past = slot * (2 * TK * LD * (uint32_t)sizeof(T));
+    ks.fetch(past, j0 * a.k_row, bits, a.dim);
+    vs.fetch(past, j0 * a.v_row, bits, a.dim);
     if (bias)
-      copy4_to_lds(lds_bias + slot * kBiasSpan + wave * kWave, bias + bias_at(a, r0 + off - j0 - (TK - 1)) + threadIdx.x);
+      copy4_to_lds(bias_to + slot * (kBiasSpan * 4), bias + bias_at(a, r0 + off - j0 - (TK - 1)) + threadIdx.x);
   };
   auto settle = [&](int slot) {
     ks.settle(lds + slot * 2 * TK * LD);
@@ -453,6 +456,9 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
   }
 
   Stage qs, gs;
+  qs.open(lds, static_cast<const T*>(a.q) + b * a.q_batch, a.q_row, a.dim);
+  gs.open(lds + TQ * LD, static_cast<const T*>(g.grad_out) + b * g.g_batch, g.g_row, a.dim);
+  const uint32_t row_to = lds_address(lds_row + wave * kWave), bias_to = lds_address(lds_bias + wave * kWave);
   int fetch_head = 0, fetch_tile = 0;  // the next pair to fetch: head of the group, tile of the walk
   auto fetch = [&](int, int slot) {
     const int head = kv * share + fetch_head, row0 = (t_first + fetch_tile) * TQ;
@@ -461,21 +467,20 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_kv_kernel(AttnCal
       ++fetch_head;
     }
     const uint64_t bits = mask.bits<TQ>(row0 + off);
-    T* to = lds + slot * 2 * TQ * LD;
-    qs.fetch(to, static_cast<const T*>(a.q) + b * a.q_batch + head * a.q_head, a.q_row, row0, bits, a.dim);
-    gs.fetch(to + TQ * LD, static_cast<const T*>(g.grad_out) + b * g.g_batch + head * g.g_head, g.g_row, row0, bits,
-             a.dim);
+    const uint32_t past = slot * (2 * TQ * LD * (uint32_t)sizeof(T));
+    qs.fetch(past, head * a.q_head + row0 * a.q_row, bits, a.dim);
+    gs.fetch(past, head * g.g_head + row0 * g.g_row, bits, a.dim);
     // one float a thread: the rows' statistics, then their delta (rows past the last one take its)
     {
       const int n = threadIdx.x, most = a.q_len - 1;
       const int r = n < 2 * TQ ? row0 + (n >> 1) : row0 + ((n - 2 * TQ) & (TQ - 1));
       const int64_t at = ((int64_t)b * a.q_heads + head) * a.q_len + (r < most ? r : most);
       const float* from = n < 2 * TQ ? reinterpret_cast<const float*>(g.stats + at) + (n & 1) : g.delta + at;
-      copy4_to_lds(lds_row + slot * kAttnThreads + wave * kWave, from);
+      copy4_to_lds(row_to + slot * (kAttnThreads * 4), from);
     }
     // lds_bias[i]: distance i + that of the tile's first query and the block's last key
     if (a.bias)
-      copy4_to_lds(lds_bias + slot * kBiasSpan + wave * kWave,
+      copy4_to_lds(bias_to + slot * (kBiasSpan * 4),
                    head_bias(a, head) + bias_at(a, row0 + off - k0 - (kAttnRows - 1)) + threadIdx.x);
   };
   auto settle = [&](int slot) {
