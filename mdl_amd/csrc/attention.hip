@@ -13,9 +13,9 @@
 // tile t + 1 is on its way while tile t is worked on.  What bounds it: the wave's
 // own chain of products, exponentials (a quarter of the vector rate) and
 // products; matrix instructions are busy about half of the time at dimension
-// 128 (8192 rows, window 1024, 16 heads: 230 us, 600 TFLOP/s) and a third at 64,
-// where a 256-key window's tiles are mostly masked (64 ragged rows of 2048:
-// 90 us).  Taking instructions out (constant starts, masks) changed little.
+// 128 (2 x 8192 rows, window 1024, 16 heads: 193 us, 710 TFLOP/s) and a third at
+// 64, where a 256-key window's tiles are mostly masked (64 ragged rows of 2048,
+// 4 heads: 82 us; 8 rows of up to 4096 without a window, 8 heads: 149).
 #include "attention.cuh"
 
 namespace mdl {
@@ -144,16 +144,8 @@ __global__ __launch_bounds__(256) void attention_prepare_kernel(PrepareCall a) {
 // (p stays below 2^8): most tiles then skip the rescaling of out.
 constexpr float kLazyRaise = 8.f;
 
-// Waves a SIMD that the registers are held to.  The narrow tiles of bf16 are
-// short of work between their waits: three waves instead of the two that free
-// registers would give took 64 x 2048 rows (4 heads of 64, window 256) from 105
-// to 90 us and 8 x 4096 without a window (8 heads on 2) from 195 to 180.
-template <typename T, int DP>
-constexpr int forward_waves() { return sizeof(T) == 2 && DP <= 64 ? 3 : 1; }
-
 template <typename T, int DP, bool kVec>
-__global__ __launch_bounds__(kAttnThreads, (forward_waves<T, DP>())) void attention_forward_kernel(AttnCall a, T* out,
-                                                                                                 float2* stats) {
+__global__ __launch_bounds__(kAttnThreads) void attention_forward_kernel(AttnCall a, T* out, float2* stats) {
   using F = Frags<T>;
   using Stage = TileStage<T, DP, kVec>;
   constexpr int TK = F::kTile, LD = Tile<T, DP>::kLd, kSteps = DP / F::kStep, kSubs = TK / 32;

@@ -17,16 +17,16 @@
 // is 0 with the true delta), and takes the share of k that belongs to the
 // difference (a fourth product, sum p k) off dq at the end; the second kernel
 // reads the corrected delta.  (The residual of out, saved by the forward, would
-// spare that product, 45 us of 490 at dimension 128, for another 2 bytes per
-// element of out held until the backward.)
+// spare that product, a tenth of the queries' kernel at dimension 128, for
+// another 2 bytes per element of out held until the backward.)
 //
-// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 130 us for
-// the queries, 165 for the keys, 42 for the first tokens' far pairs; 2 x 8192
-// rows (16 heads of 128 on 4, window 1024): 485, 540 and 45.  At dimension 128
+// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 124 us for
+// the queries, 160 for the keys, 42 for the first tokens' far pairs; 2 x 8192
+// rows (16 heads of 128 on 4, window 1024): 423, 497 and 45.  At dimension 128
 // the accumulators leave room for one wave a SIMD, whose chain of LDS reads,
-// products and exponentials bounds it (matrix instructions 30 % of the time);
-// two waves spill (540 for the queries), and the products of one sub-tile under
-// the exponentials of another took longer (466 against 433, both without sum p k).
+// products and exponentials bounds it (matrix instructions a third of the time);
+// two waves spill (an eighth longer), and the products of one sub-tile under the
+// exponentials of another took longer too (466 against 433, without sum p k).
 #include "attention.cuh"
 
 namespace mdl {
@@ -205,8 +205,8 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 // columns are summed by the lanes into four registers each (64 distances of
 // which a tile fills 63).  Along the walk the next tile's distances lie 32
 // further: half of the sums are complete, cross the lanes and are stored, the
-// other half moves down.  (One LDS addition per value instead cost 356 us
-// where the kernel's products cost 159.)  Tiles wholly in the last bucket
+// other half moves down.  (One LDS addition per value instead took 356 us
+// where the whole kernel takes 160.)  Tiles wholly in the last bucket
 // are summed into one register.
 
 struct DiagonalSums {
