@@ -331,10 +331,16 @@ __device__ __forceinline__ uint32_t lds_address(void* lds) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void)lds);
 }
 __device__ __forceinline__ void copy16_to_lds(uint32_t lds, const void* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(from)
+               : "memory");
 }
 __device__ __forceinline__ void copy4_to_lds(uint32_t lds, const void* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(from)
+               : "memory");
 }
 
 // All but the wave's last kLeft memory operations have ended: the copies
@@ -388,7 +394,7 @@ struct TileStage {
   // to its first row; bits: the live ones.  Scalar offsets from the thread's own
   // place, and no selection where every row is live: with an address made from
   // its row for each piece the walks were a seventh longer (2 x 8192 rows of 16
-  // heads of 128: 229, 484 and 545 us, now 193, 423 and 497).
+  // heads of 128: 229, 484 and 545 us, with it 193, 423 and 497).
   __device__ __forceinline__ void fetch(uint32_t past, int64_t first, uint64_t bits, int D) {
     const T* from = mine + first;
     if (kDirect && full && bits == ~0ull) {

@@ -16,13 +16,17 @@
 // all the same, adds the row's dS in fp32 to what it is short of (their sum
 // is 0 with the true delta), and takes the share of k that belongs to the
 // difference (a fourth product, sum p k) off dq at the end; the second kernel
-// reads the corrected delta.  (The residual of out, saved by the forward, would
+// reads the corrected delta.  Delta is taken off after the product dP, not put
+// in as its start: dP is then the same in every kernel and the difference exact
+// where the two are close, so a row that sees one key has dS = 0 to the bit (its
+// dq is set to 0, since the first kernel's dS still holds the first delta).
+// (The residual of out, saved by the forward, would
 // spare that product, a tenth of the queries' kernel at dimension 128, for
 // another 2 bytes per element of out held until the backward.)
 //
-// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 124 us for
-// the queries, 160 for the keys, 42 for the first tokens' far pairs; 2 x 8192
-// rows (16 heads of 128 on 4, window 1024): 423, 497 and 45.  At dimension 128
+// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 128 us for
+// the queries, 161 for the keys, 42 for the first tokens' far pairs; 2 x 8192
+// rows (16 heads of 128 on 4, window 1024): 445, 500 and 45.  At dimension 128
 // the accumulators leave room for one wave a SIMD, whose chain of LDS reads,
 // products and exponentials bounds it (matrix instructions a third of the time);
 // two waves spill (an eighth longer), and the products of one sub-tile under the
@@ -49,14 +53,6 @@ struct GradCall {
 constexpr int kSpare = 96;      // distances of one tile and wave past either end of the bias
 constexpr int kFarRows = 256;   // query rows of a block of the first tokens' far part
 constexpr int kSkew = 64;       // diagonals of a 32x32 product tile, padded
-
-// Whether dP is computed alone and delta taken off it afterwards, instead of
-// dP starting there (one instruction less).  In fp32 the difference is then exact
-// where the two are close, and dP the same in every kernel: a row that sees one
-// key has dS = 0 to the bit, and sums of dS over such rows (the first of every
-// history) stay 0.  bf16 results do not resolve that.
-template <typename T>
-constexpr bool late_delta() { return sizeof(T) == 4; }
 
 // ------------------------------------------------------ queries: dq, delta --
 
@@ -116,6 +112,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = pk[i] = (f32x16)(0.f);
   float rest = 0.f;  // sum of dS: delta less dO . out
+  uint32_t others = 0;  // not 0: the row sees a key beside its own
   const float far_bias = bias ? load_uniform(bias + kBiasEdge + a.distances - 1) : 0.f;
   // scores start at the bias less the maximum; a large maximum is taken off at the end
   const bool large = bias && is_large(a, m_neg), any_large = __any(large);
@@ -149,9 +146,10 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
     const bool far = !bias || wc_lo - j1 >= a.distances - 1;
     const bool whole = q_bits == ~0u && (TK == 64 ? bits == ~0ull : (uint32_t)bits == ~0u) && j1 <= wc_lo &&
                        wc_lo + 31 - j0 < a.window && !any_large;
+    if (whole) others = 1;
 #pragma unroll
     for (int s = 0; s < kSubs; ++s) {
-      f32x16 x, dp = (f32x16)(late_delta<T>() ? 0.f : -delta);
+      f32x16 x, dp = (f32x16)(0.f);
       if (far) {
         x = (f32x16)(far_from);
       } else {
@@ -170,6 +168,8 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
       if (!whole) {
         if (any_large) x = (x + (far && large ? far_bias : 0.f)) + (large ? m_neg : 0.f);
         uint32_t vis = live ? visible32(c, j0 + 32 * s, a.window, walk.sink_end, (uint32_t)(bits >> (32 * s))) : 0u;
+        const uint32_t own = c - (j0 + 32 * s);
+        others |= vis & ~(own < 32 ? 1u << own : 0u);
         vis >>= 4 * half;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = keep_bit(vis, 8 * (i >> 2) + (i & 3), x[i], -INFINITY);
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, ll_neg));
-        dp[i] = (late_delta<T>() ? dp[i] - delta : dp[i]) * x[i];
+        dp[i] = (dp[i] - delta) * x[i];
         rest += dp[i];
       }
       // p and dS take the element type for the products with k
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_q_kernel(AttnCall
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[dt][i] = __builtin_fmaf(-rest, pk[dt][i], acc[dt][i]);
+    for (int i = 0; i < 16; ++i) acc[dt][i] = others ? __builtin_fmaf(-rest, pk[dt][i], acc[dt][i]) : 0.f;
   store_result_row<T, DP>(static_cast<T*>(g.dq) + (((int64_t)b * a.q_len + row) * a.q_heads + head) * a.dim, acc,
                           a.scale, a.dim);
 }
@@ -301,11 +301,10 @@ struct KeyTile {
     const bool any_large = a.bias && __any(is_large(a, stats[2 * (lane_id() & 31)]));
     stats += 8 * half;
     delta += 4 * half;
-    f32x16 x, dp;
+    f32x16 x, dp = (f32x16)(0.f);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       x[i] = stats[2 * (8 * (i >> 2) + (i & 3))];
-      dp[i] = late_delta<T>() ? 0.f : delta[8 * (i >> 2) + (i & 3)];
     }
     if (near_bias) {
 #pragma unroll
@@ -343,7 +342,7 @@ struct KeyTile {
     for (int i = 0; i < 16; ++i) x[i] = exp2_fast(__builtin_fmaf(x[i], a.c2, stats[2 * (8 * (i >> 2) + (i & 3)) + 1]));
     gt.times(x, dv);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= late_delta<T>() ? dp[i] + delta[8 * (i >> 2) + (i & 3)] : dp[i];
+    for (int i = 0; i < 16; ++i) x[i] *= dp[i] + delta[8 * (i >> 2) + (i & 3)];
     qt.times(x, dk);
     return x;
   }

@@ -216,6 +216,18 @@ def test_attention_repeats_itself_and_follows_its_stream(device):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Lq,Lk,window,D", [(1, 1, None, 64), (150, 150, 1, 64), (90, 100, 1, 24), (70, 70, 1, 128)])
+def test_one_visible_key_gives_no_score_gradient(device, dtype, Lq, Lk, window, D):
+    """p is 1 whatever the score: dq, dk and the bias's gradient are 0 to the bit."""
+
+    announce("one key", dtype, Lq, Lk, window, D)
+    got = run_attention(device, dtype, 2, Lq, Lk, 4, 2, D, None if Lq == 1 else holes(4, 2, Lk, "holes"), window, 0,
+                        (8, 24))
+    for g in (got[1], got[2], got[4]):
+        assert not g.any()
+
+
 def test_attention_against_differences(device):
     # fp32: the loss moves by step^2 of its third derivative (about 1e-4 here)
     # and by its own rounding, 1e-6 / step, of a directional derivative of order 10
