@@ -10,6 +10,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -36,6 +37,15 @@ Tensor inner_contiguous(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1
 
 void same_device(const Tensor& t, const Tensor& q, const char* what) {
   TORCH_CHECK_VALUE(t.device() == q.device(), what, " must live on the queries' device");
+}
+
+// The operators have no forward-mode formulas, and run below autograd where
+// nothing requires a gradient: a dual input would lose its tangent there, so
+// it is refused.
+template <typename... Inputs>
+void refuse_tangents(const char* what, const Inputs&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(torch::autograd::isFwGradDefined(inputs) || ...), what,
+                              " has no forward-mode derivative");
 }
 
 // ------------------------------------------------------------- attention --
@@ -227,6 +237,7 @@ struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
 Tensor history_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& mask,
                                   const std::optional<Tensor>& bias_table, const std::optional<Tensor>& bucket_starts,
                                   int64_t distances, int64_t window, int64_t sinks, double scale) {
+  refuse_tangents("history_attention", q, k, v, bias_table);
   const bool need = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                    (bias_table.has_value() && bias_table->requires_grad()));
   if (need) return HistoryAttention::apply(q, k, v, mask, bias_table, bucket_starts, distances, window, sinks, scale);
@@ -416,6 +427,7 @@ struct RelativeBias : public torch::autograd::Function<RelativeBias> {
 
 Tensor relative_bias_autograd(const Tensor& table, const Tensor& starts, bool bidirectional, int64_t q_len,
                               int64_t k_len) {
+  refuse_tangents("relative_position_bias", table);
   if (at::GradMode::is_enabled() && table.requires_grad())
     return RelativeBias::apply(table, starts, bidirectional, q_len, k_len);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -580,6 +592,7 @@ std::tuple<Tensor, Tensor> block_norm_autograd(const Tensor& x, const std::optio
                                                const std::optional<Tensor>& post_weight, const Tensor& next_weight,
                                                const std::optional<Tensor>& gate,
                                                const std::optional<Tensor>& residual_scale, double eps) {
+  refuse_tangents("gated_residual_norm", x, block_out, post_weight, next_weight, gate, residual_scale);
   auto wants = [](const std::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
   if (at::GradMode::is_enabled() && (x.requires_grad() || next_weight.requires_grad() || wants(block_out) ||
                                      wants(post_weight) || wants(gate) || wants(residual_scale))) {
