@@ -10,9 +10,12 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <string>
 #include <tuple>
 
 #include "../../include/mdl_hip.h"
@@ -46,6 +49,21 @@ template <typename... Inputs>
 void refuse_tangents(const char* what, const Inputs&... inputs) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(torch::autograd::isFwGradDefined(inputs) || ...), what,
                               " has no forward-mode derivative");
+}
+
+// The gradients have no formula of their own: under create_graph they lead to
+// a node that raises when it is differentiated, on the way to whatever they
+// were made from (saved inputs, upstream gradients).
+variable_list differentiable_once(const char* what, variable_list grads, const variable_list& saved,
+                                  const variable_list& upstream) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto edges = torch::autograd::collect_next_edges(saved, upstream);
+  if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) return grads;
+  const auto node = std::make_shared<torch::autograd::Error>(
+      std::string(what) + " can be differentiated once: its gradients have no derivative", std::move(edges));
+  for (const Tensor& g : grads)
+    if (g.defined()) torch::autograd::set_history(g, node);
+  return grads;
 }
 
 // ------------------------------------------------------------- attention --
@@ -230,7 +248,9 @@ struct HistoryAttention : public torch::autograd::Function<HistoryAttention> {
                 ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble(), s[6], s[7], s[8],
                 need_table);
     const Tensor none;
-    return {dq, dk, dv, none, need_table ? dtable : none, none, none, none, none, none};
+    return differentiable_once("history_attention",
+                               {dq, dk, dv, none, need_table ? dtable : none, none, none, none, none, none},
+                               {s[0], s[1], s[2], s[4]}, grads);
   }
 };
 
@@ -419,9 +439,11 @@ struct RelativeBias : public torch::autograd::Function<RelativeBias> {
                                .findSchemaOrThrow("mdl_hip::relative_position_bias_backward", "")
                                .typed<decltype(relative_bias_grad_cuda)>();
     const Tensor none;
-    return {op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["buckets"].toInt(),
-                    ctx->saved_data["bidirectional"].toBool()),
-            none, none, none, none};
+    return differentiable_once("relative_position_bias",
+                               {op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["buckets"].toInt(),
+                                        ctx->saved_data["bidirectional"].toBool()),
+                                none, none, none, none},
+                               {}, grads);
   }
 };
 
@@ -582,8 +604,10 @@ struct BlockNorm : public torch::autograd::Function<BlockNorm> {
     auto [dx, d_o, dgate, dscale, dpost, dnext] =
         op.call(optional_of(dy), optional_of(dh), s[0], optional_of(s[1]), optional_of(s[2]), s[3], optional_of(s[4]),
                 optional_of(s[5]), s[6], ctx->saved_data["eps"].toDouble(), needs);
-    return {dx, two ? d_o : none, needs & 2 ? dpost : none, needs & 4 ? dnext : none, s[4].defined() ? dgate : none,
-            needs & 1 ? dscale : none, none};
+    return differentiable_once("gated_residual_norm",
+                               {dx, two ? d_o : none, needs & 2 ? dpost : none, needs & 4 ? dnext : none,
+                                s[4].defined() ? dgate : none, needs & 1 ? dscale : none, none},
+                               {s[0], s[1], s[2], s[3], s[4], s[5]}, grads);
   }
 };
 

@@ -60,3 +60,47 @@ def test_a_tangent_is_refused(name, requires_grad):
         call(t)  # a plain tensor inside the level is as good as outside
     with pytest.raises(RuntimeError):
         torch.func.jvp(call, (rand(*shape),), (torch.ones(shape),))
+
+
+@pytest.mark.parametrize("name", INPUTS)
+def test_a_second_derivative_raises(name):
+    """First gradients are right under create_graph too; what would go through
+    them again raises, instead of leaving its part out."""
+
+    call, shape = INPUTS[name]
+    t = rand(*shape).requires_grad_()
+    plain = torch.autograd.grad(call(t).square().sum(), t)[0]
+    (grad,) = torch.autograd.grad(call(t).square().sum(), t, create_graph=True)
+    assert torch.equal(grad.detach(), plain)
+    with pytest.raises(RuntimeError, match="once"):
+        (grad.square().sum() + t.sum()).backward()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(grad.square().sum() + t.sum(), t)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.functional.hvp(lambda x: call(x).square().sum(), rand(*shape), torch.ones(shape))
+
+
+def test_a_second_derivative_raises_for_what_only_the_gradients_share():
+    # k requires nothing of its own: the upstream gradient alone leads back to w
+    w = rand(2, 5, 4, 3).requires_grad_()
+    q = rand(2, 5, 4, 3).requires_grad_()
+    (grad,) = torch.autograd.grad((_attention(q=q) * w).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(grad.sum(), w)
+
+
+def test_a_gradient_that_depends_on_nothing_differentiable_is_a_constant():
+    # the bias is linear in its table, and this upstream gradient is given
+    table = rand(6, 4).requires_grad_()
+    (grad,) = torch.autograd.grad(relative_position_bias(table, 4, 5, RULE), table, rand(4, 4, 5), create_graph=True)
+    assert not grad.requires_grad
+
+
+def test_what_does_not_pass_the_operators_twice_is_left_alone():
+    # a penalty on another branch of the same graph
+    q, a = rand(2, 5, 4, 3).requires_grad_(), rand(3).requires_grad_()
+    loss = _attention(q=q).sum() + a.pow(3).sum()
+    dq, da = torch.autograd.grad(loss, [q, a], create_graph=True)
+    da.square().sum().backward()
+    torch.testing.assert_close(a.grad, 36 * a.detach() ** 3)
+    assert dq.requires_grad and q.grad is None
