@@ -74,9 +74,21 @@ class RelativeBuckets:
         return f"RelativeBuckets({self.num_buckets}, {self.max_distance}, bidirectional={self.bidirectional})"
 
     def starts_on(self, device: torch.device) -> Tensor:
-        t = self._on_device.get(device)
+        """The starts as a tensor, kept for later calls.  What is kept serves
+        any of them: never an inference tensor, and nothing made under a
+        dispatch mode (fake tensors, tracing), a functional transform or in a
+        compiled graph, where each call without a kept one makes its own."""
+
+        if torch.compiler.is_dynamo_compiling():
+            t = self._on_device.get(device)
+            return torch.tensor(self.starts, dtype=torch.int32, device=device) if t is None else t
+        moded = torch._C._len_torch_dispatch_stack() > 0  # a kept tensor is foreign to fake ones
+        t = None if moded else self._on_device.get(device)
         if t is None:
-            t = self._on_device[device] = torch.tensor(self.starts, dtype=torch.int32, device=device)
+            with torch.inference_mode(False):
+                t = torch.tensor(self.starts, dtype=torch.int32, device=device)
+            if not moded and torch._C._functorch.peek_interpreter_stack() is None:
+                self._on_device[device] = t
         return t
 
     @property
