@@ -299,6 +299,13 @@ mdl_attention_step cache_args(const Tensor& k, const Tensor& v, const Tensor& ca
   return a;
 }
 
+// The kernels write the cache through its address: autograd learns of it here,
+// as an in-place operation of its own would tell it.
+void cache_changed(const Tensor& cache_k, const Tensor& cache_v) {
+  for (const Tensor* t : {&cache_k, &cache_v})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void check_positions(const Tensor& t, const Tensor& cache, const char* what) {
   TORCH_CHECK_TYPE(t.scalar_type() == at::kLong, what, " must be torch.long");
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == cache.size(0), what, " must hold one entry per row of the cache");
@@ -349,6 +356,7 @@ Tensor cache_step_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if (bytes) ws = empty_on(q, {(int64_t)bytes}, at::kByte);
   check(mdl_attention_step_forward(&a, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q.device())),
         "mdl_attention_step_forward");
+  cache_changed(cache_k, cache_v);
   return out;
 }
 
@@ -368,6 +376,7 @@ void cache_write_cuda(const Tensor& k, const Tensor& v, const Tensor& cache_k, c
   check(mdl_attention_cache_write(&a, k.size(1), ki.stride(1), vi.stride(1), static_cast<const int64_t*>(ln.data_ptr()),
                                   right_aligned ? 1 : 0, stream_of(k.device())),
         "mdl_attention_cache_write");
+  cache_changed(cache_k, cache_v);
 }
 
 // --------------------------------------------------- relative position bias --
