@@ -333,6 +333,13 @@ def _cache_step_cpu(q, k, v, cache_k, cache_v, positions, bias_table, bucket_sta
         _check_bias(bias_table, bucket_starts, distances, q.size(1))
     if B == 0:
         return torch.empty_like(q)
+    with torch._C._AutoDispatchBelowAutograd():  # operations of PyTorch, of which nothing is recorded
+        return _stored_and_answered_cpu(q, k, v, cache_k, cache_v, positions, bias_table, bucket_starts, window, sinks,
+                                        scale)
+
+
+def _stored_and_answered_cpu(q, k, v, cache_k, cache_v, positions, bias_table, bucket_starts, window, sinks, scale):
+    B, capacity, K, D = cache_k.shape
     held, at = _cache_rows_cpu(positions, capacity, sinks)
     row = (positions >= 0).nonzero().flatten()
     cache_k[row, at[row]] = k[row]
@@ -369,13 +376,14 @@ def _cache_write_cpu(k, v, cache_k, cache_v, lengths, sinks, right_aligned):
         raise ValueError("a prompt's k and v must be [B, L, Hkv, D] of the cache's rows")
     _check_positions(lengths, cache_k, "lengths")
     ring, L = capacity - sinks, k.size(1)
-    for b in range(B):
-        n = min(int(lengths[b]), L)
-        p = torch.arange(max(n, 0))
-        p = p[(p < sinks) | (p >= n - ring)]
-        slots = torch.where(p < sinks, p, sinks + (p - sinks) % ring)
-        rows = p + (L - n if right_aligned else 0)
-        cache_k[b, slots], cache_v[b, slots] = k[b, rows], v[b, rows]
+    with torch._C._AutoDispatchBelowAutograd():  # as for a step
+        for b in range(B):
+            n = min(int(lengths[b]), L)
+            p = torch.arange(max(n, 0))
+            p = p[(p < sinks) | (p >= n - ring)]
+            slots = torch.where(p < sinks, p, sinks + (p - sinks) % ring)
+            rows = p + (L - n if right_aligned else 0)
+            cache_k[b, slots], cache_v[b, slots] = k[b, rows], v[b, rows]
 
 
 @_fake_kernel("history_cache_write_")
