@@ -761,7 +761,9 @@ int mdl_attention_step_forward(const mdl_attention_step* step, void* out, void* 
  * and head strides of the descriptor, row strides k_row and v_row) hold each
  * row's positions 0 .. lengths[b] - 1 in their first rows, or their last ones
  * with right_aligned; those that no later position of the same slot replaces
- * are stored.  q, positions and the bias of the descriptor are not used. */
+ * are stored.  A length above len counts as len (a caller that goes on from the
+ * true length checks first), a negative one as 0.  q, positions and the bias of
+ * the descriptor are not used. */
 int mdl_attention_cache_write(const mdl_attention_step* step, int64_t len, int64_t k_row, int64_t v_row,
                               const int64_t* lengths, int32_t right_aligned, void* stream);
 

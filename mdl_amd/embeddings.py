@@ -108,8 +108,8 @@ def check_index_errors() -> None:
         if bad:
             counter.zero_()
             raise IndexError(
-                f"{bad} embedding lookups or bag poolings received out-of-range IDs "
-                f"or inconsistent bag lengths on {device}"
+                f"{bad} embedding lookups, bag poolings or history prompts received out-of-range IDs "
+                f"or inconsistent bag or prompt lengths on {device}"
             )
 
 

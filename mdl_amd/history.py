@@ -33,6 +33,7 @@ import torch
 from torch import Tensor
 
 from . import library  # noqa: F401  (loads libmdl_torch.so and its schemas)
+from .embeddings import _deferred_counter, index_check_mode
 from .library import _cpu_kernel, _fake_kernel
 
 # the operators' overloads, looked up once
@@ -376,9 +377,11 @@ def _cache_write_cpu(k, v, cache_k, cache_v, lengths, sinks, right_aligned):
         raise ValueError("a prompt's k and v must be [B, L, Hkv, D] of the cache's rows")
     _check_positions(lengths, cache_k, "lengths")
     ring, L = capacity - sinks, k.size(1)
+    if bool((lengths > L).any()):
+        raise ValueError(f"history cache lengths must not exceed the prompt's {L} rows")
     with torch._C._AutoDispatchBelowAutograd():  # as for a step
         for b in range(B):
-            n = min(int(lengths[b]), L)
+            n = int(lengths[b])
             p = torch.arange(max(n, 0))
             p = p[(p < sinks) | (p >= n - ring)]
             slots = torch.where(p < sinks, p, sinks + (p - sinks) % ring)
@@ -505,6 +508,18 @@ def relative_position_bias(table: Tensor, q_len: int, k_len: int, buckets: Relat
     return _BIAS(table, buckets.starts_on(table.device), buckets.bidirectional, int(q_len), int(k_len))
 
 
+def _check_lengths(lengths: Tensor, rows: int) -> None:
+    message = f"history cache lengths must not exceed the prompt's {rows} rows"
+    mode = index_check_mode()
+    if mode == "sync":
+        if bool((lengths > rows).any()):
+            raise ValueError(message)
+    elif mode == "deferred":
+        _deferred_counter(lengths.device).add_((lengths > rows).sum())
+    else:
+        torch._assert_async((lengths <= rows).all(), message)
+
+
 class HistoryCache:
     """Keys and values of histories that grow, one row per user.
 
@@ -544,8 +559,13 @@ class HistoryCache:
     def write(self, k: Tensor, v: Tensor, lengths: Tensor, *, right_aligned: bool = False) -> None:
         """Store prompts: ``k, v [B, L, Hkv, D]`` hold positions ``0 ..
         lengths[b] - 1`` of each row in their first rows, or in their last
-        ones (``sequence_embedding_lookup``'s window) with ``right_aligned``."""
+        ones (``sequence_embedding_lookup``'s window) with ``right_aligned``.
+        A length above ``L`` is refused, on a ROCm device as out-of-range ids
+        are (``embeddings.set_index_check_mode``): the rows it misses would be
+        answered from all the same.  A negative one stores nothing."""
 
+        if lengths.is_cuda and k.ndim == 4:
+            _check_lengths(lengths, k.size(1))
         _WRITE(k, v, self.k, self.v, lengths, self.sinks, right_aligned)
 
     def step(self, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, *, bias_table: Optional[Tensor] = None,

@@ -5,6 +5,7 @@ biases swallow."""
 import pytest
 import torch
 
+from mdl_amd.embeddings import check_index_errors, index_check_mode, set_index_check_mode
 from mdl_amd.history import HistoryCache, RelativeBuckets, history_attention
 from tests import history_reference as R
 from tests.test_gpu_history import announce, make
@@ -45,3 +46,30 @@ def test_a_cache_of_inference_tensors_takes_steps(device):
     at = torch.tensor([3, 2], device=device)
     assert torch.equal(cache.step(q[:, 0], q[:, 1], q[:, 2], at), outside.step(q[:, 0], q[:, 1], q[:, 2], at))
     assert torch.equal(cache.k, outside.k)
+
+
+def test_a_length_past_the_prompt_is_refused(device):
+    # "async", the default, would trap the device: only lengths that pass are written under it
+    announce("long lengths")
+    k = make(0, F32, 2, 5, 2, 16).to(device)
+    cache = HistoryCache.empty(2, 16, 2, 16, device=device)
+    good, bad = torch.tensor([5, -1], device=device), torch.tensor([5, 6], device=device)
+    mode = index_check_mode()
+    try:
+        set_index_check_mode("sync")
+        with pytest.raises(ValueError, match="5 rows"):
+            cache.write(k, k, bad)
+        assert not cache.k.any()
+        cache.write(k, k, good)
+        set_index_check_mode("deferred")
+        cache.write(k, k, good)
+        check_index_errors()
+        cache.write(k, k, bad)
+        with pytest.raises(IndexError, match="^1 .*history prompts"):
+            check_index_errors()
+        set_index_check_mode("async")
+        cache.write(k, k, good)
+        torch.cuda.synchronize()
+    finally:
+        set_index_check_mode(mode)
+    assert torch.equal(cache.k[0, :5], k[0])

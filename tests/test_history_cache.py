@@ -1,5 +1,7 @@
-"""The cache of histories on the CPU: what its steps leave behind."""
+"""The cache of histories on the CPU: what its steps leave behind and what its
+writes refuse."""
 
+import pytest
 import torch
 
 from mdl_amd.history import HistoryCache
@@ -39,3 +41,23 @@ def test_blocks_step_without_no_grad():
         for block, cache in zip(enc.blocks, caches):
             block.step(x, x, torch.tensor([t, t]), cache)
             assert cache.k.grad_fn is None and cache.v.grad_fn is None
+
+
+@pytest.mark.parametrize("right", [False, True])
+def test_a_length_past_the_prompt_is_refused(right):
+    """Nothing is stored: a step at the true length would answer from rows that
+    were never written."""
+
+    cache = HistoryCache.empty(3, 16, 2, 4)
+    k, v = rand(3, 5, 2, 4), rand(3, 5, 2, 4)
+    with pytest.raises(ValueError, match="5 rows"):
+        cache.write(k, v, torch.tensor([2, 6, 1]), right_aligned=right)
+    assert not cache.k.any() and not cache.v.any()
+    cache.write(k, v, torch.tensor([5, 0, -2]), right_aligned=right)
+    assert cache.k[0, :5].ne(0).all() and not cache.k[1:].any()
+
+
+def test_prefill_refuses_lengths_past_its_columns():
+    enc = _encoder()
+    with pytest.raises(ValueError, match="9 rows"):
+        enc.prefill(torch.ones(2, 9, dtype=torch.long), torch.tensor([4, 11]), enc.caches(2))
