@@ -53,6 +53,8 @@ struct AttnCall {
   float scale;
 };
 
+__device__ __forceinline__ int clamp_to(int v, int most) { return v < 0 ? 0 : (v < most ? v : most); }
+
 // ------------------------------------------------------------- fragments --
 
 template <typename T>

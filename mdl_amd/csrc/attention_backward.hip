@@ -380,8 +380,9 @@ struct BlockBias {
     float* partial = g.bias_partial + ((int64_t)head * g.bias_parts + part) * g.buckets;
     const int sub = threadIdx.x & 7;
     for (int k = threadIdx.x >> 3; k < g.buckets; k += kAttnThreads / 8) {
-      const int lo = k == 0 ? 0 : g.starts[k - 1];
-      const int hi = k == g.buckets - 1 ? a.distances + kSpare - 4 : g.starts[k];
+      const int most = a.distances + kSpare - 4;  // the sums end there, whatever the starts hold
+      const int lo = k == 0 ? 0 : clamp_to(g.starts[k - 1], most);
+      const int hi = k == g.buckets - 1 ? most : clamp_to(g.starts[k], most);
       float s = 0.f;
       for (int d = lo + sub; d < hi; d += 8) s += sums[d - shift + kSpare];
       for (int x = 4; x >= 1; x >>= 1) s += __shfl_xor(s, x);

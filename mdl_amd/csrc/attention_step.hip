@@ -244,10 +244,11 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall 
       }
       lds_table[i] = v;
     }
-    // bucket by bucket: every distance from its start to the next one's
+    // bucket by bucket: every distance from its start to the next one's (of the
+    // distances told apart: starts and their number are arguments of their own)
     for (int k = wave; k < a.buckets; k += kWaves) {
-      const int from = k == 0 ? 0 : a.starts[k - 1];
-      const int to = k == a.buckets - 1 ? a.distances : a.starts[k];
+      const int from = k == 0 ? 0 : clamp_to(a.starts[k - 1], a.distances);
+      const int to = k == a.buckets - 1 ? a.distances : clamp_to(a.starts[k], a.distances);
       for (int x = from + lane_id(); x < to; x += kWave) lds_bucket[x] = (uint16_t)k;
     }
     __syncthreads();

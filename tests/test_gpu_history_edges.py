@@ -73,3 +73,39 @@ def test_a_length_past_the_prompt_is_refused(device):
     finally:
         set_index_check_mode(mode)
     assert torch.equal(cache.k[0, :5], k[0])
+
+
+def _raw(device, dtype, starts, distances, D=32, H=8):
+    """Outputs and gradients of the operators themselves, whose starts and
+    number of distances are separate arguments."""
+
+    q, k, v = (make(i, dtype, 2, 90, h, D).to(device) for i, h in ((0, H), (1, 1), (2, 1)))
+    table = make(3, dtype, len(starts) + 1, H).to(device)
+    starts = torch.tensor(starts, dtype=torch.int32, device=device)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = torch.ops.mdl_hip.history_attention(*leaves[:3], None, table, starts, distances, 20, 3, 0.2)
+    got = [out.detach(), *torch.autograd.grad(out.float().square().sum(), leaves)]
+    with torch.no_grad():
+        cache = HistoryCache.empty(2, 128, 1, D, dtype=dtype, device=device)
+        cache.write(k, v, torch.tensor([90, 60], device=device))
+        got.append(torch.ops.mdl_hip.history_cache_step(
+            q[:, 0], k[:, 0], v[:, 0], cache.k, cache.v, torch.tensor([90, 60], device=device), table, starts, distances,
+            100, 0, 0.2))
+    return got
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_starts_past_the_distances_stay_in_bounds(device, dtype):
+    """Starts that do not fit the distances told apart make no promise for the
+    bias, but nothing outside the kernels' sums and buckets is touched: what
+    runs after them is as if they had not."""
+
+    announce("starts past distances", dtype)
+    rule = list(RelativeBuckets(8, 24).starts)
+    want = _raw(device, dtype, rule, rule[-1] + 1)
+    for starts, distances in (([5, 300, 2000, 30000, 2**31 - 1, 2**31 - 1, 2**31 - 1], 3), (rule, 1),
+                              ([-2**31, -40000, -7, 0, 1, 2, 3], 4)):
+        for t in _raw(device, dtype, starts, distances):
+            assert torch.isfinite(t).all(), (starts, distances)
+    for a, b in zip(_raw(device, dtype, rule, rule[-1] + 1), want):
+        assert torch.equal(a, b)
