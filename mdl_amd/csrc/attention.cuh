@@ -588,7 +588,8 @@ __device__ __forceinline__ uint32_t visible32(int c, int col, int window, int si
 int attention_check(const mdl_attention* a, const char* what);
 AttnCall attention_call(const mdl_attention& a, const void* prepared);
 bool attention_vectors(const mdl_attention& a);  // 16-byte rows throughout
-int allow_lds(const void* kernel, size_t bytes);
+// Lets a kernel have `dynamic` bytes of LDS beside its own `fixed` ones.
+int allow_lds(const void* kernel, size_t dynamic, size_t fixed = 0);
 
 // Calls f.template operator()<T, DP, kVec>() with the element type, the head
 // dimension rounded up to 32, 64 or 128 (the columns past it are zeros in LDS

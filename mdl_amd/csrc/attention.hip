@@ -396,9 +396,9 @@ bool attention_vectors(const mdl_attention& a) {
          whole(a.v, a.v_batch, a.v_row, a.v_head);
 }
 
-int allow_lds(const void* kernel, size_t bytes) {
-  if (bytes <= 64 * 1024) return MDL_OK;
-  return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+int allow_lds(const void* kernel, size_t dynamic, size_t fixed) {
+  if (dynamic + fixed <= 64 * 1024) return MDL_OK;
+  return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic),
                    "hipFuncSetAttribute");
 }
 

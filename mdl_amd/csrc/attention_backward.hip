@@ -53,6 +53,7 @@ struct GradCall {
 constexpr int kSpare = 96;      // distances of one tile and wave past either end of the bias
 constexpr int kFarRows = 256;   // query rows of a block of the first tokens' far part
 constexpr int kSkew = 64;       // diagonals of a 32x32 product tile, padded
+constexpr int kFarFlats = 4;    // sums of the far part's waves in the last bucket
 
 // ------------------------------------------------------ queries: dq, delta --
 
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_grad_far_kernel(AttnCa
   float* lr = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + kWalk * 64 * LD) + wave * (96 + kBias);
   float* lb = lr + 96;  // lr: (-m, -log2 sum)[32], -delta[32]
   float* joined = reinterpret_cast<float*>(smem);  // [dk, dv][32][dim], after the walk
-  __shared__ float flats[4];
+  __shared__ float flats[kFarFlats];
 
   const int share = a.q_heads / a.kv_heads, off = a.k_len - a.q_len;
   const int key_blocks = (a.sinks + 31) / 32;
@@ -764,7 +765,7 @@ int launch_backward(const AttnCall& a, const GradCall& g, hipStream_t s) {
     const size_t lds = walk > join ? walk : join;
     const auto kernel = attention_grad_far_kernel<T, DP, kVec>;
     if (blocks > 0x7fffffff) return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_backward: too many rows");
-    if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+    if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds, kFarFlats * sizeof(float))) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kAttnThreads), lds, s, a, g);
     MDL_CHECK_LAUNCH("attention_grad_far_kernel");
   }

@@ -155,6 +155,12 @@ __device__ __forceinline__ void store_piece(T* row, int d, int D, const float* v
 template <int G>
 constexpr int few_blocks() { return G == 8 ? 256 : 512; }
 
+// What a block's waves leave for its join: (maximum, sum, values) of a lane's
+// piece and head.  Beside the bias the largest shape (fp32, 8 heads a row of
+// more than 64, 1024 buckets over 2049 distances) takes 84 KB of LDS in all.
+template <typename T, int L, int G, int kWaves>
+using StepJoin = float[kWaves][L][G][Frags<T>::kElems + 2];
+
 template <typename T, int L, int G, bool kVec, int kWaves>
 __global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall a, T* out) {
   using F = Frags<T>;
@@ -163,7 +169,7 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall 
   extern __shared__ __align__(16) char smem[];
   float* lds_table = reinterpret_cast<float*>(smem);           // [buckets][G] bias in powers of two
   uint16_t* lds_bucket = reinterpret_cast<uint16_t*>(lds_table + a.buckets * G);  // [distances]
-  __shared__ float lds_join[kWaves][L][G][E + 2];
+  __shared__ StepJoin<T, L, G, kWaves> lds_join;
 
   const int share = a.q_heads / a.kv_heads, groups = (share + G - 1) / G;
   unsigned id = blockIdx.x;
@@ -540,7 +546,7 @@ template <typename T, int L, int G, bool kVec, int kWaves>
 int launch_step(const StepCall& c, int64_t blocks, void* out, hipStream_t s) {
   const size_t lds = ((size_t)c.buckets * G * 4 + (size_t)c.distances * 2 + 15) & ~size_t(15);
   const auto kernel = attention_step_kernel<T, L, G, kVec, kWaves>;
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return rc;
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), lds, sizeof(StepJoin<T, L, G, kWaves>))) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * kWave), lds, s, c, static_cast<T*>(out));
   MDL_CHECK_LAUNCH("attention_step_kernel");
   return MDL_OK;

@@ -8,7 +8,7 @@ import torch
 from mdl_amd.embeddings import check_index_errors, index_check_mode, set_index_check_mode
 from mdl_amd.history import HistoryCache, RelativeBuckets, history_attention
 from tests import history_reference as R
-from tests.test_gpu_history import announce, make
+from tests.test_gpu_history import announce, holes, make, run_attention, run_steps
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,36 @@ def test_starts_past_the_distances_stay_in_bounds(device, dtype):
             assert torch.isfinite(t).all(), (starts, distances)
     for a, b in zip(_raw(device, dtype, rule, rule[-1] + 1), want):
         assert torch.equal(a, b)
+
+
+# the most buckets and distances that an attention takes: 1024 of them, the last from 2048 on
+LARGEST = RelativeBuckets(1024, 2053)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_attention_with_the_largest_rule(device, monkeypatch, dtype, D):
+    """The keys' and the far part's kernels at the most LDS that they take."""
+
+    assert LARGEST.starts[-1] == 2048
+    monkeypatch.setattr(R, "bucket", lambda distance, *_: LARGEST.of(distance))
+    run_attention(device, dtype, 1, 2200, 2200, 2, 1, D, None, 700, 40, (1024, 2053))
+    run_attention(device, dtype, 1, 300, 2200, 2, 2, D, holes(4, 1, 2200, "holes"), None, 0, (1024, 2053))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("max_distance", [798, 804, 806, 807, 810])
+def test_attention_around_64_kb_of_lds(device, monkeypatch, dtype, max_distance):
+    # rules of 660 to 680 distances at head dimension 32: the far part's LDS passes 64 KB among them
+    rule = RelativeBuckets(40, max_distance)
+    monkeypatch.setattr(R, "bucket", lambda distance, *_: rule.of(distance))
+    run_attention(device, dtype, 1, 800, 800, 1, 1, 32, None, 200, 5, (40, max_distance))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,D", [(8, 128), (8, 64), (2, 128), (12, 128)])
+@pytest.mark.parametrize("B", [1, 300])
+def test_step_with_the_largest_rule(device, monkeypatch, dtype, H, D, B):
+    monkeypatch.setattr(R, "bucket", lambda distance, *_: LARGEST.of(distance))
+    lengths = [2250] if B == 1 else [3 * (i % 20) for i in range(B)]
+    run_steps(device, dtype, lengths, 2304 if B == 1 else 64, None, 0, H, 1, D, (1024, 2053), steps=1)
