@@ -327,21 +327,18 @@ __device__ __forceinline__ void load_own_row(const T* row, bool live, int D,
 // to lds + 16 l or 4 l (lds: one address per wave).  It holds no register;
 // wait_fetched ends it.  Written out because the compiler, which knows the
 // instruction, would wait for it before any transposing read of LDS,
-// whichever buffer that reads.
+// whichever buffer that reads; m0, which holds the place, stays the compiler's
+// to set (a wait state lies between).
 __device__ __forceinline__ uint32_t lds_address(void* lds) {
   typedef __attribute__((address_space(3))) void* lds_void;
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void)lds);
 }
 __device__ __forceinline__ void copy16_to_lds(uint32_t lds, const void* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
-                   __builtin_amdgcn_readfirstlane(lds)),
-               "v"(from)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(lds)), "v"(from)
                : "memory");
 }
 __device__ __forceinline__ void copy4_to_lds(uint32_t lds, const void* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
-                   __builtin_amdgcn_readfirstlane(lds)),
-               "v"(from)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(lds)), "v"(from)
                : "memory");
 }
 
