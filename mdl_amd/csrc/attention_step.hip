@@ -441,17 +441,18 @@ __global__ __launch_bounds__(kJoinThreads) void attention_step_join_kernel(StepC
 
 // The prompt form: rows of k and v at positions 0 .. length - 1 take their
 // slots, those that a later one of the same slot replaces left out.  One
-// block per (batch row, 64 rows); a thread moves elements of one row.
+// block per (batch row, kWriteRows rows); a thread moves elements of one row.
+constexpr int kWriteRows = 64;
 template <typename T>
-__global__ __launch_bounds__(256) void cache_write_kernel(StepCall a, int64_t len, const int64_t* lengths,
-                                                           int32_t right_aligned) {
-  const int b = blockIdx.y;
+__global__ __launch_bounds__(256) void cache_write_kernel(StepCall a, int64_t len, uint32_t blocks_per_row,
+                                                           const int64_t* lengths, int32_t right_aligned) {
+  const int b = (int)(blockIdx.x / blocks_per_row);
   int64_t n = lengths[b];
   if (n > len) n = len;
   const int64_t shift = right_aligned ? len - n : 0;
   const int width = a.kv_heads * a.dim;
-  const int64_t r0 = (int64_t)blockIdx.x * 64;
-  for (int64_t i = threadIdx.x; i < 64 * (int64_t)width; i += 256) {
+  const int64_t r0 = (int64_t)(blockIdx.x % blocks_per_row) * kWriteRows;
+  for (int64_t i = threadIdx.x; i < kWriteRows * (int64_t)width; i += 256) {
     const int64_t r = r0 + i / width, p = r - shift;
     const int c = (int)(i % width), kv = c / a.dim, d = c % a.dim;
     if (r >= len || p < 0 || p >= n) continue;
@@ -632,18 +633,19 @@ int mdl_attention_cache_write(const mdl_attention_step* a, int64_t len, int64_t 
   if (int rc = step_check(&with, "mdl_attention_cache_write")) return rc;
   if (len < 0) return fail(MDL_ERR_INVALID, "mdl_attention_cache_write: negative length");
   if (a->batch == 0 || len == 0) return MDL_OK;
-  if (a->batch > 65535 || (len + 63) / 64 > 0x7fffffff)
+  const int64_t per_row = (len - 1) / kWriteRows + 1;
+  if (per_row > 0x7fffffff / a->batch)
     return fail(MDL_ERR_UNSUPPORTED, "mdl_attention_cache_write: too many rows");
   StepCall c = step_call(with);
   c.row_k = k_row;
   c.row_v = v_row;
-  const dim3 grid((unsigned)((len + 63) / 64), (unsigned)a->batch);
+  const dim3 grid((unsigned)(per_row * a->batch));
   if (a->dtype == MDL_BF16)
-    hipLaunchKernelGGL(cache_write_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream), c, len, lengths,
-                       right_aligned);
+    hipLaunchKernelGGL(cache_write_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream), c, len,
+                       (uint32_t)per_row, lengths, right_aligned);
   else
-    hipLaunchKernelGGL(cache_write_kernel<float>, grid, dim3(256), 0, as_stream(stream), c, len, lengths,
-                       right_aligned);
+    hipLaunchKernelGGL(cache_write_kernel<float>, grid, dim3(256), 0, as_stream(stream), c, len,
+                       (uint32_t)per_row, lengths, right_aligned);
   MDL_CHECK_LAUNCH("cache_write_kernel");
   return MDL_OK;
 }

@@ -142,3 +142,21 @@ def test_step_with_the_largest_rule(device, monkeypatch, dtype, H, D, B):
     monkeypatch.setattr(R, "bucket", lambda distance, *_: LARGEST.of(distance))
     lengths = [2250] if B == 1 else [3 * (i % 20) for i in range(B)]
     run_steps(device, dtype, lengths, 2304 if B == 1 else 64, None, 0, H, 1, D, (1024, 2053), steps=1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_users_than_a_grid_is_high(device, dtype):
+    """A write takes the batches that a step takes: 70,000 rows, of two blocks each."""
+
+    announce("many users", dtype)
+    B, L, D = 70000, 66, 4
+    k = torch.arange(B * L, dtype=torch.float32).remainder(251).reshape(B, L, 1, 1).expand(B, L, 1, D).to(dtype).to(device)
+    lengths = torch.arange(B, device=device) % (L + 1)
+    cache = HistoryCache.empty(B, L + 1, 1, D, dtype=dtype, device=device)
+    cache.write(k, -k, lengths, right_aligned=True)
+    column = torch.arange(L, device=device)
+    rows = (column + L - lengths[:, None]).clamp(max=L - 1)
+    want = torch.where((column < lengths[:, None])[..., None], k[:, :, 0].gather(1, rows[..., None].expand(B, L, D)), 0.0)
+    assert torch.equal(cache.k[:, :L, 0], want.to(dtype)) and torch.equal(cache.v, -cache.k)
+    one = torch.ones(B, 1, D, dtype=dtype, device=device)
+    assert cache.step(one, one, one, lengths).shape == (B, 1, D)
