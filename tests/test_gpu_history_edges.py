@@ -160,3 +160,35 @@ def test_more_users_than_a_grid_is_high(device, dtype):
     assert torch.equal(cache.k[:, :L, 0], want.to(dtype)) and torch.equal(cache.v, -cache.k)
     one = torch.ones(B, 1, D, dtype=dtype, device=device)
     assert cache.step(one, one, one, lengths).shape == (B, 1, D)
+
+
+@pytest.mark.parametrize("name", ["attention", "attention_forward", "step", "write", "bias", "norm"])
+def test_opcheck(device, name):
+    announce("opcheck", name)
+    ops = torch.ops.mdl_hip
+    grad = name not in ("step", "write", "attention_forward")
+    q, k, v = (make(i, F32, 2, 9, h, 8).to(device).requires_grad_(grad) for i, h in ((0, 4), (1, 2), (2, 2)))
+    table = make(3, F32, 6, 4).to(device).requires_grad_(grad)
+    rule = RelativeBuckets(6, 8)
+    starts, mask = rule.starts_on(q.device), holes(1, 2, 9, "holes").to(device)
+    bias = (table, starts, rule.distances)
+    if name == "attention":
+        torch.library.opcheck(ops.history_attention.default, (q, k, v, mask, *bias, 3, 1, 0.5))
+    elif name == "attention_forward":
+        # its third result is the call's prepared buffer, whose padding holds anything: values are not compared
+        torch.library.opcheck(ops.history_attention_forward.default, (q, k, v, mask, *bias, 3, 1, 0.5, True),
+                              test_utils=("test_schema", "test_faketensor"))
+    elif name == "step":
+        torch.library.opcheck(ops.history_cache_step.default,
+                              (q[:, 0], k[:, 0], v[:, 0], k.clone(), v.clone(), torch.tensor([1, 5], device=device), *bias,
+                               3, 1, 0.5), test_utils=("test_schema", "test_faketensor"))
+    elif name == "write":
+        torch.library.opcheck(ops.history_cache_write_.default,
+                              (k, v, k.clone(), v.clone(), torch.tensor([2, 9], device=device), 1, True),
+                              test_utils=("test_schema", "test_faketensor"))
+    elif name == "bias":
+        torch.library.opcheck(ops.relative_position_bias.default, (table, starts, False, 4, 9))
+    else:
+        x, o, gate = (make(i, F32, 3, 8).to(device).requires_grad_() for i in range(3))
+        w = [make(4 + i, F32, 8).to(device).requires_grad_() for i in range(3)]
+        torch.library.opcheck(ops.gated_residual_norm.default, (x, o, w[0], w[1], gate, w[2], 1e-6))
