@@ -12,10 +12,11 @@
 // dimension 128), where rows lie for both readings without bank conflicts, and
 // tile t + 1 is on its way while tile t is worked on.  What bounds it: the wave's
 // own chain of products, exponentials (a quarter of the vector rate) and
-// products; matrix instructions are busy about half of the time at dimension
-// 128 (2 x 8192 rows, window 1024, 16 heads: 193 us, 710 TFLOP/s) and a third at
-// 64, where a 256-key window's tiles are mostly masked (64 ragged rows of 2048,
-// 4 heads: 82 us; 8 rows of up to 4096 without a window, 8 heads: 149).
+// products; matrix instructions are busy 36 % of the time at dimension 128
+// (2 x 8192 rows, window 1024, 16 heads: 178 us, 735 TFLOP/s), 22 % at 64 without
+// a window (8 rows of up to 4096, 8 heads: 147 us) and 14 % at 64 with one of 256
+// keys, where half of the waves' tiles are partly masked (64 ragged rows of
+// 2048, 4 heads: 84 us).
 #include "attention.cuh"
 
 namespace mdl {

@@ -18,19 +18,24 @@
 // difference (a fourth product, sum p k) off dq at the end; the second kernel
 // reads the corrected delta.  Delta is taken off after the product dP, not put
 // in as its start: dP is then the same in every kernel and the difference exact
-// where the two are close, so a row that sees one key has dS = 0 to the bit (its
-// dq is set to 0, since the first kernel's dS still holds the first delta).
+// where the two are close, so in a row that sees one key dP - delta comes to 0.
+// (Unless the terms of that row's dP cancel to a millionth of their size: p, made
+// again from the score, need not be 1 exactly, and up to 2^-40 or so of the terms
+// can be left.  Its dq is set to 0, since the first kernel's dS still holds the
+// first delta.)
 // (The residual of out, saved by the forward, would
 // spare that product, a tenth of the queries' kernel at dimension 128, for
 // another 2 bytes per element of out held until the backward.)
 //
-// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 128 us for
-// the queries, 161 for the keys, 42 for the first tokens' far pairs; 2 x 8192
-// rows (16 heads of 128 on 4, window 1024): 445, 500 and 45.  At dimension 128
+// Times: 64 ragged rows of 2048 (4 heads of 64, window 256, bias): 126 us for
+// the queries, 158 for the keys, 41 for the first tokens' far pairs; 2 x 8192
+// rows (16 heads of 128 on 4, window 1024): 414, 467 and 44.  At dimension 128
 // the accumulators leave room for one wave a SIMD, whose chain of LDS reads,
-// products and exponentials bounds it (matrix instructions a third of the time);
-// two waves spill (an eighth longer), and the products of one sub-tile under the
-// exponentials of another took longer too (466 against 433, without sum p k).
+// products and exponentials bounds it (matrix instructions are busy 29 % of the
+// time for the queries and 23 % for the keys); at 64 it is the same chain with two
+// blocks a CU (17 % and 11 %).  At 128 two waves spill (an eighth longer), and
+// the products of one sub-tile under the exponentials of another took longer
+// too (466 against 433, without sum p k).
 #include "attention.cuh"
 
 namespace mdl {

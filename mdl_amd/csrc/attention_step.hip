@@ -8,9 +8,11 @@
 // walks every (groups of the block)-th row with its own running maximum and
 // sum; groups, then waves, then blocks are joined at the end.  Few rows with
 // long caches are cut into parts over several blocks, joined by a second
-// launch.  256 users with up to 1028 rows of 64 (103 MB): 27.8 us, 3.7 TB/s, the
-// longest walks bound it; two users with 62,000 rows of 128 (129 MB): 26 and
-// 4 us, 4.2 TB/s together.
+// launch.  256 users with up to 1028 rows of 64 (103 MB): 31 us, 3.3 TB/s, the
+// longest walks bound it; two users with 62,000 rows of 128 (129 MB): 31 and
+// 5 us, 3.6 TB/s together.  (Of caches that other data has driven out of the
+// last-level cache, as a model's other layers do.  The figures beside the rules
+// below are of loops over two states, of which part stays there: 28, and 26 and 4.)
 #include "attention.cuh"
 
 namespace mdl {
@@ -19,7 +21,8 @@ constexpr int kJoinThreads = 1024;
 // A walk is cut where few of them would leave CUs idle; joining the parts
 // costs a launch of 4 to 5 us.  (bf16 caches of 1028 rows of 64, 8 query
 // heads on 2 key heads: one user 17 us whole, 16.5 in parts of 512 rows, 13.8
-// in four of 257; 100 users, 200 walks: 18.5 whole, 24.6 in two.)
+// in four of 257; 100 users, 200 walks: 18.5 whole, 24.6 in two.  Longer caches
+// were not measured between kCutUnits walks and one for every CU.)
 constexpr int kStepBlocks = 512;   // blocks wanted of walks that are cut
 constexpr int kCutUnits = 128;     // walks above which none is cut
 constexpr int kStepMinRows = 256;  // cached rows of a part at least
@@ -371,7 +374,8 @@ __global__ __launch_bounds__(kWaves* kWave) void attention_step_kernel(StepCall 
 // Joins the parts of a row's walk: one block per row and head.  Waves take every
 // kWaves-th part, kAtOnce of them with all loads on their way at once and no
 // load waiting for a maximum: the parts come from other XCDs, a trip of about
-// a microsecond (128 parts of 16 rows: 4.2 us; 13 with the maximum first).
+// a microsecond (128 parts, two users of 8 heads of 128: 4.2 us; 13 with the
+// maximum first).
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void attention_step_join_kernel(StepCall a, T* out) {
   constexpr int kWaves = kJoinThreads / kWave, kAtOnce = 8;

@@ -8,7 +8,7 @@
 // The backward makes y again from x, o and gate (y as it was before rounding)
 // instead of reading it: the same bytes, since x would have to be read with it
 // for nothing else.  Bytes bound both directions: 262144 rows of 256 in bf16
-// take 134 us forward and 203 backward, 5.0 and 5.3 TB/s, the rate of a copy.
+// take 133 us forward and 210 backward, 5.0 and 5.1 TB/s, the rate of a copy.
 //
 // A row lies in the registers of a group of lanes (4 to 256, as wide as it
 // needs); its two sums are taken across the group.  Sums over rows (the

@@ -15,8 +15,11 @@ rows and ``[B, T]`` mask, projected to heads, attend to each other.
 The operators are ``mdl_hip::history_attention`` (differentiable) over
 ``history_attention_forward`` and ``history_attention_backward``,
 ``history_cache_step``, ``history_cache_write_`` and
-``relative_position_bias`` (over its ``_forward`` and ``_backward``): ROCm kernels in ``libmdl_torch.so`` over the C ABI, CPU kernels (PyTorch operations, for
-parameters on the CPU) and fake kernels registered here.
+``relative_position_bias`` (over its ``_forward`` and ``_backward``): ROCm
+kernels in ``libmdl_torch.so`` over the C ABI, CPU kernels (PyTorch operations,
+for parameters on the CPU) and fake kernels registered here.  The differentiable
+ones have first gradients only: a dual input is refused, and so is what would
+differentiate a gradient.
 
 The mask marks a row's real columns.  A masked column is neither read as a key
 nor answered as a query: its output and gradients are zeros whatever its rows
@@ -529,7 +532,8 @@ class HistoryCache:
     ``capacity == sinks + window`` a row keeps just what its next token sees,
     however long its history.
 
-    Inference only: nothing here is differentiable.
+    Inference only: nothing here is differentiable, and nothing is recorded.
+    Steps and writes change ``k`` and ``v`` in place, which autograd learns of.
     """
 
     def __init__(self, k: Tensor, v: Tensor, *, window: Optional[int] = None, sinks: int = 0) -> None:
