@@ -77,15 +77,13 @@ class RelativeBuckets:
     def __repr__(self) -> str:
         return f"RelativeBuckets({self.num_buckets}, {self.max_distance}, bidirectional={self.bidirectional})"
 
+    @torch.compiler.assume_constant_result  # a compiled graph takes the kept tensor
     def starts_on(self, device: torch.device) -> Tensor:
         """The starts as a tensor, kept for later calls.  What is kept serves
         any of them: never an inference tensor, and nothing made under a
-        dispatch mode (fake tensors, tracing), a functional transform or in a
-        compiled graph, where each call without a kept one makes its own."""
+        dispatch mode (fake tensors, tracing) or a functional transform, where
+        each call makes its own."""
 
-        if torch.compiler.is_dynamo_compiling():
-            t = self._on_device.get(device)
-            return torch.tensor(self.starts, dtype=torch.int32, device=device) if t is None else t
         moded = torch._C._len_torch_dispatch_stack() > 0  # a kept tensor is foreign to fake ones
         t = None if moded else self._on_device.get(device)
         if t is None:

@@ -192,3 +192,22 @@ def test_opcheck(device, name):
         x, o, gate = (make(i, F32, 3, 8).to(device).requires_grad_() for i in range(3))
         w = [make(4 + i, F32, 8).to(device).requires_grad_() for i in range(3)]
         torch.library.opcheck(ops.gated_residual_norm.default, (x, o, w[0], w[1], gate, w[2], 1e-6))
+
+
+def test_a_rule_first_compiled_under_inference_trains(device):
+    announce("compiled rule")
+    rule = RelativeBuckets(6, 8)
+
+    def attend(q, table):
+        return history_attention(q, q[:, :, :2], q[:, :, 2:], window=3, bias_table=table, buckets=rule)
+
+    compiled = torch.compile(attend, backend="aot_eager", fullgraph=True)
+    q, table = make(0, F32, 2, 5, 4, 8).to(device), make(1, F32, 6, 4).to(device)
+    with torch.inference_mode():
+        first = compiled(q, table)
+    leaves = [t.clone().requires_grad_() for t in (q, table)]
+    for call in (attend, compiled):
+        out = call(*leaves)
+        assert torch.equal(out, first)
+        grads = torch.autograd.grad(out.square().sum(), leaves)
+        assert all(torch.isfinite(g).all() and g.any() for g in grads)

@@ -77,6 +77,9 @@ def test_a_rule_first_used_in_a_compiled_function_works_outside():
         q, table = rand(2, 5, 4, 3), rand(6, 4)
         with torch.inference_mode(inference):
             compiled(q, table)
+        # the graph holds the kept tensor and makes none of its own
+        kept = rule._on_device[q.device]
+        assert type(kept) is torch.Tensor and not kept.is_inference() and kept.tolist() == list(rule.starts)
         torch.testing.assert_close(compiled(q, table), attend(RelativeBuckets(6, 8), q, table))
         train(rule)
 
