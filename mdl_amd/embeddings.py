@@ -95,7 +95,8 @@ _DEFERRED_COUNTERS: dict[torch.device, Tensor] = {}
 def _deferred_counter(device: torch.device) -> Tensor:
     t = _DEFERRED_COUNTERS.get(device)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # counts outside inference mode too
+            t = torch.zeros(1, dtype=torch.int32, device=device)
         _DEFERRED_COUNTERS[device] = t
     return t
 

@@ -97,3 +97,18 @@ def test_an_encoder_that_answered_first_trains_afterwards():
         e(ids, lengths)[0].sum().backward()
     for a, b in zip(enc.parameters(), other.parameters()):
         assert torch.equal(a.grad.to_dense(), b.grad.to_dense())
+
+
+def test_the_deferred_counter_first_used_in_inference_mode_counts_outside(monkeypatch):
+    """Lookups and prompt writes of an evaluation make it; a later step outside
+    inference mode adds to it and resets it."""
+
+    from mdl_amd import embeddings
+
+    monkeypatch.setattr(embeddings, "_DEFERRED_COUNTERS", {})
+    with torch.inference_mode():
+        embeddings._deferred_counter(torch.device("cpu")).add_(1)
+    embeddings._deferred_counter(torch.device("cpu")).add_(1)
+    with pytest.raises(IndexError, match="^2 "):
+        embeddings.check_index_errors()
+    embeddings.check_index_errors()
